@@ -62,8 +62,20 @@ class LossSet(ctypes.Structure):
               ('mode', ctypes.c_int32)]
 
 
+class AttentionArgs(ctypes.Structure):
+  _fields_ = [
+      ('q', ctypes.c_void_p), ('k', ctypes.c_void_p), ('v', ctypes.c_void_p),
+      ('q_stride', ctypes.c_int64 * 3), ('k_stride', ctypes.c_int64 * 3), ('v_stride', ctypes.c_int64 * 3),
+      ('padding', ctypes.c_void_p), ('padding_stride', ctypes.c_int64),
+      ('dtype', ctypes.c_int32), ('B', ctypes.c_int32), ('L', ctypes.c_int32), ('S', ctypes.c_int32),
+      ('H', ctypes.c_int32), ('G', ctypes.c_int32), ('D', ctypes.c_int32), ('causal', ctypes.c_int32),
+      ('scale', ctypes.c_float), ('out', ctypes.c_void_p), ('lse', ctypes.c_void_p), ('dout', ctypes.c_void_p),
+      ('dout_stride', ctypes.c_int64 * 3), ('dq', ctypes.c_void_p), ('dk', ctypes.c_void_p), ('dv', ctypes.c_void_p),
+      ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t)]
+
+
 _lib = None
-ABI_VERSION = 401          # HSGK_VERSION the struct layouts / signatures below were written for
+ABI_VERSION = 402          # HSGK_VERSION the struct layouts / signatures below were written for
 
 _vp, _i64, _i32, _f32, _sz = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
                               ctypes.c_float, ctypes.c_size_t)
@@ -118,6 +130,11 @@ SIGNATURES = {
     'hsgk_topk_workspace_bytes': (_sz, [_i64, _i32, _i64, _i32]),
     'hsgk_topk_prototypes': (_i32, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _sz, _vp]),
     'hsgk_topk_prototypes_grouped': (_i32, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'hsgk_attention_workspace_bytes': (_sz, [ctypes.POINTER(AttentionArgs), _i32]),
+    'hsgk_attention_fwd': (_i32, [ctypes.POINTER(AttentionArgs), _vp]),
+    'hsgk_attention_bwd': (_i32, [ctypes.POINTER(AttentionArgs), _vp]),
+    'hsgk_topk_distill_fwd': (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp]),
+    'hsgk_topk_distill_bwd': (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _vp]),
     'hsgk_synth_gaussish': (_i32, [ctypes.c_uint64, ctypes.c_uint64, _i64, _vp, _vp]),
     'hsgk_synth_mixture': (_i32, [ctypes.c_uint64, ctypes.c_uint64, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     'hsgk_assign_workspace_bytes': (_sz, [_i64, _i32, _i32]),

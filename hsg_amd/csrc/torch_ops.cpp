@@ -25,6 +25,11 @@
 //       hsg/models/embeddings/resnet_fcn_hsg.py:499-577, :638-672, :683-748, :751-780: the padded per-image tables,
 //       the two-level assignment (+ its one-launch backward), the masked group means (+ hsgk_group_mean_bwd) and
 //       the pixel -> group lookup -- one dispatch each, outputs allocated here.
+//   hsgk::attention(q, k, v, padding?, causal, scale) -> out
+//       what hsg/models/heads/transformer.py gets from torch.nn.MultiheadAttention between its projections; the backward
+//       recomputes the probabilities from q, k and the saved row statistics.
+//   hsgk::topk_distill(logits, teacher, index, temperature) -> loss per row
+//       distillation from the teacher's k best prototypes, gradient for the logits.
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -655,6 +660,158 @@ std::tuple<Tensor, Tensor> dmon_pool(const Tensor &adj, const Tensor &s, const c
   return {r[0], r[1]};
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// attention: q [B,L,H,D], k / v [B,S,G,D] (checked by hsg_amd/ops.py), padding bool [B,S] or none
+int type_code(const Tensor &t) {
+  return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2;
+}
+
+Tensor last_contiguous(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+void set_strides(int64_t (&st)[3], const Tensor &t) {
+  for (int i = 0; i < 3; ++i) st[i] = t.stride(i);
+}
+
+hsgk_attention_args attention_args(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &pad, bool causal,
+                                   double scale, const Tensor &out) {
+  hsgk_attention_args a{};
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+  set_strides(a.q_stride, q); set_strides(a.k_stride, k); set_strides(a.v_stride, v);
+  if (pad.defined() && pad.numel()) {
+    a.padding = static_cast<const uint8_t *>(pad.data_ptr());
+    a.padding_stride = pad.stride(0);
+  }
+  a.dtype = type_code(q);
+  a.B = (int32_t)q.size(0); a.L = (int32_t)q.size(1); a.H = (int32_t)q.size(2); a.D = (int32_t)q.size(3);
+  a.S = (int32_t)k.size(1); a.G = (int32_t)k.size(2);
+  a.causal = causal; a.scale = (float)scale;
+  a.out = out.data_ptr();
+  return a;
+}
+
+Tensor attention_fwd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &pad, bool causal, double scale, Tensor *lse) {
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor out = at::empty(q.sizes(), q.options());
+  hsgk_attention_args a = attention_args(q, k, v, pad, causal, scale, out);
+  if (lse) {
+    *lse = at::empty({q.size(0), k.size(2), q.size(1), q.size(2) / k.size(2)}, q.options().dtype(at::kFloat));
+    a.lse = lse->data_ptr<float>();
+  }
+  Tensor ws;
+  if (const size_t wsb = hsgk_attention_workspace_bytes(&a, 0)) {
+    ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = wsb;
+  }
+  check(hsgk_attention_fwd(&a, stream_of(q)), "hsgk_attention_fwd");
+  return out;
+}
+
+struct AttentionFn : public torch::autograd::Function<AttentionFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &pad, bool causal,
+                        double scale) {
+    Tensor lse, out = attention_fwd(q, k, v, pad, causal, scale, &lse);
+    ctx->save_for_backward({q, k, v, pad, out, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &pad = sv[3], &out = sv[4], &lse = sv[5];
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    Tensor g = last_contiguous(grads[0]);
+    Tensor dq = at::empty(q.sizes(), q.options()), dk, dv;
+    hsgk_attention_args a = attention_args(q, k, v, pad, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), out);
+    a.lse = lse.data_ptr<float>();
+    a.dout = g.data_ptr();
+    set_strides(a.dout_stride, g);
+    a.dq = dq.data_ptr();
+    const bool want_k = ctx->needs_input_grad(1), want_v = ctx->needs_input_grad(2);
+    if (want_k || want_v) {
+      dk = at::empty(k.sizes(), k.options());
+      dv = at::empty(v.sizes(), v.options());
+      a.dk = dk.data_ptr();
+      a.dv = dv.data_ptr();
+    }
+    Tensor ws;
+    if (const size_t wsb = hsgk_attention_workspace_bytes(&a, 1)) {
+      ws = at::empty({(int64_t)wsb}, q.options().dtype(at::kByte));
+      a.workspace = ws.data_ptr();
+      a.workspace_bytes = wsb;
+    }
+    check(hsgk_attention_bwd(&a, stream_of(q)), "hsgk_attention_bwd");
+    return {dq, want_k ? dk : Tensor(), want_v ? dv : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, const c10::optional<Tensor> &padding, bool causal, double scale) {
+  TORCH_CHECK(q.is_cuda(), "hsgk::attention: tensors must be on a ROCm device (there is no CPU path)");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
+                  q.size(3) == k.size(3) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
+                  (q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) &&
+                  k.device() == q.device() && v.device() == q.device(),
+              "hsgk::attention: q [B,L,H,D], k and v [B,S,G,D] of one floating type on one device");
+  Tensor pad = padding.has_value() && padding->defined() ? *padding : Tensor();
+  if (pad.defined()) {
+    TORCH_CHECK(pad.dim() == 2 && pad.size(0) == k.size(0) && pad.size(1) == k.size(1) && pad.scalar_type() == at::kBool &&
+                    pad.device() == q.device(), "hsgk::attention: padding is bool [B,S] on the tensors' device");
+    pad = last_contiguous(pad);
+  } else {
+    pad = at::empty({0}, q.options().dtype(at::kBool));
+  }
+  const Tensor qc = last_contiguous(q), kc = last_contiguous(k), vc = last_contiguous(v);
+  if (at::GradMode::is_enabled() && (qc.requires_grad() || kc.requires_grad() || vc.requires_grad()))
+    return AttentionFn::apply(qc, kc, vc, pad, causal, scale);
+  return attention_fwd(qc, kc, vc, pad, causal, scale, nullptr);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// distillation from a teacher's k best classes: logits [n,V], teacher float32 [n,k], index int64 [n,k] -> loss [n]
+Tensor distill_fwd(const Tensor &z, const Tensor &t, const Tensor &idx, double temperature, Tensor *stats) {
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(z.device());
+  Tensor loss = at::empty({z.size(0)}, t.options());
+  if (stats) *stats = at::empty({z.size(0), 2}, t.options());
+  check(hsgk_topk_distill_fwd(z.data_ptr(), type_code(z), z.size(0), z.size(1), z.stride(0), t.data_ptr<float>(),
+                              idx.data_ptr<int64_t>(), (int)t.size(1), (float)temperature, loss.data_ptr<float>(),
+                              stats ? stats->data_ptr<float>() : nullptr, stream_of(z)),
+        "hsgk_topk_distill_fwd");
+  return loss;
+}
+
+struct TopkDistillFn : public torch::autograd::Function<TopkDistillFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &z, const Tensor &t, const Tensor &idx, double temperature) {
+    Tensor stats, loss = distill_fwd(z, t, idx, temperature, &stats);
+    ctx->save_for_backward({z, t, idx, stats});
+    ctx->saved_data["temperature"] = temperature;
+    return loss;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &z = sv[0], &t = sv[1], &idx = sv[2], &stats = sv[3];
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(z.device());
+    Tensor g = grads[0].to(at::kFloat).contiguous();
+    Tensor dz = at::empty(z.sizes(), z.options());
+    check(hsgk_topk_distill_bwd(z.data_ptr(), type_code(z), z.size(0), z.size(1), z.stride(0), t.data_ptr<float>(),
+                                idx.data_ptr<int64_t>(), (int)t.size(1), (float)ctx->saved_data["temperature"].toDouble(),
+                                stats.data_ptr<float>(), g.data_ptr<float>(), dz.data_ptr(), stream_of(z)),
+          "hsgk_topk_distill_bwd");
+    return {dz, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor topk_distill(const Tensor &logits, const Tensor &teacher, const Tensor &index, double temperature) {
+  TORCH_CHECK(logits.is_cuda(), "hsgk::topk_distill: tensors must be on a ROCm device (there is no CPU path)");
+  TORCH_CHECK(logits.dim() == 2 && teacher.dim() == 2 && teacher.sizes() == index.sizes() && teacher.size(0) == logits.size(0) &&
+                  (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf) &&
+                  teacher.scalar_type() == at::kFloat && index.scalar_type() == at::kLong &&
+                  teacher.device() == logits.device() && index.device() == logits.device(),
+              "hsgk::topk_distill: logits [n,V], teacher float32 [n,k] and index int64 [n,k] on one device");
+  const Tensor z = last_contiguous(logits), t = teacher.contiguous(), idx = index.contiguous();
+  if (at::GradMode::is_enabled() && z.requires_grad()) return TopkDistillFn::apply(z, t, idx, temperature);
+  return distill_fwd(z, t, idx, temperature, nullptr);
+}
+
 int64_t abi_version() { return hsgk_version(); }
 
 }  // namespace
@@ -674,6 +831,8 @@ TORCH_LIBRARY(hsgk, m) {
   m.def("gather_labels(Tensor table, Tensor img, Tensor seg) -> Tensor", &gather_labels);
   m.def("pad_prototype_tables(Tensor seg_image, Tensor protos, Tensor? pos, Tensor seg_lab, Tensor seg_batch,"
         " Tensor pixel_seg, int B, int M) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", &pad_prototype_tables);
+  m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? padding, bool causal, float scale) -> Tensor", &attention);
+  m.def("topk_distill(Tensor logits, Tensor teacher, Tensor index, float temperature) -> Tensor", &topk_distill);
   m.def("segment_by_kmeans(Tensor x, Tensor? labels, Tensor loc, int loc_batch_stride, Tensor seed_map,"
         " int seed_batch_stride, int K, bool has_ignore, int ignore_index, int iterations, int batch_offset,"
         " int table_cap, int flags) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)", &segment_by_kmeans);

@@ -4,8 +4,109 @@
 (`hsgk_cluster_topk`).  The transformer stack and the two FC + BN heads are the module's own
 (stock PyTorch-ROCm); `forward` below is bound onto the reference class by
 `hsg_amd.patch_reference()` or inherited through `TransformerClusteringMixin`.
+
+`attention` is the operator between the projections of the stack's attention modules
+(hsg/models/heads/transformer.py builds them from torch.nn.MultiheadAttention), forward and backward on libhsgk;
+`use_attention_kernels(module)` switches the attention modules of a built stack over to it.
 """
+import math
+
+import torch
+import torch.nn.functional as F
+
+from hsg_amd import ops
 from hsg_amd.models.embeddings import hierarchy
+
+MAX_HEAD_WIDTH = 128    # include/hsgk.h HSGK_ATTENTION_MAX_WIDTH
+
+
+def attention(query, key, value, key_padding_mask=None, is_causal=False, scale=None):
+  """softmax(scale * query key^T) value per head, differentiable in the three.
+
+  query [B, L, H, D], key and value [B, S, G, D] with H a multiple of G (query head h uses key head h // (H // G)), all
+  float32, bfloat16 or float16 with D <= 128, on one ROCm device; any strides (a last dimension that is not contiguous
+  is copied).  key_padding_mask [B, S] bool: True = not a key, as in torch.nn.MultiheadAttention; such keys and values
+  may hold anything, NaN included.  is_causal: query i sees the keys j <= i + S - L (the last query sees every key).
+  scale: positive, 1 / sqrt(D) when None.  Returns [B, L, H, D], contiguous, of the inputs' type.
+
+  A query that sees no key has output 0 and passes no gradient (torch's softmax gives NaN there).  Sums, statistics and
+  probabilities are float32; the backward pass recomputes the probabilities, uses no atomics and repeats bit for bit.
+  Under graph capture take gradients with torch.autograd.grad, which adds nothing to leaves that another graph holds.
+  """
+  for name, t in (('query', query), ('key', key), ('value', value)):
+    if t.dim() != 4:
+      raise ValueError('%s must be [batch, length, heads, width] (got %d dimensions)' % (name, t.dim()))
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16) or t.dtype is not query.dtype:
+      raise TypeError('query, key and value must share one type of float32, bfloat16, float16 (%s is %s)' % (name, t.dtype))
+    if t.device != query.device:
+      raise ValueError('query, key and value must be on one device')
+  B, _, H, D = query.shape
+  if key.shape != value.shape:
+    raise ValueError('key and value must have the same shape: %s and %s' % (tuple(key.shape), tuple(value.shape)))
+  if key.shape[0] != B or key.shape[3] != D:
+    raise ValueError('query and key disagree on the batch or the head width: %s and %s'
+                     % (tuple(query.shape), tuple(key.shape)))
+  G = key.shape[2]
+  if G < 1 or H < 1 or H % G:
+    raise ValueError('the query heads (%d) must be a multiple of the key heads (%d)' % (H, G))
+  if not 1 <= D <= MAX_HEAD_WIDTH:
+    raise ValueError('the head width must be 1 .. %d (got %d)' % (MAX_HEAD_WIDTH, D))
+  if key_padding_mask is not None:
+    if key_padding_mask.dtype is not torch.bool:
+      raise TypeError('key_padding_mask must be bool (got %s)' % key_padding_mask.dtype)
+    if tuple(key_padding_mask.shape) != (B, key.shape[1]) or key_padding_mask.device != query.device:
+      raise ValueError('key_padding_mask must be [%d, %d] on the device of the keys' % (B, key.shape[1]))
+  scale = D ** -0.5 if scale is None else float(scale)
+  if not (scale > 0.0 and math.isfinite(scale)):
+    raise ValueError('scale must be positive and finite (got %r)' % scale)
+  ops.require_gpu(query, 'query')
+  return ops.attention(query, key, value, key_padding_mask, bool(is_causal), scale)
+
+
+class MultiheadAttention(torch.nn.MultiheadAttention):
+  """torch.nn.MultiheadAttention (same parameters, state_dict and call) whose softmax(q k^T) v runs in libhsgk.  Returns
+  (output, None): the probabilities are never stored, so there are no weights to return.  A call that needs what the
+  kernels do not offer raises: attn_mask, dropout in training, bias_k / bias_v, add_zero_attn, unbatched inputs."""
+
+  def forward(self, query, key, value, key_padding_mask=None, need_weights=False, attn_mask=None,
+              average_attn_weights=True, is_causal=False):
+    if attn_mask is not None:
+      raise ValueError('MultiheadAttention: attn_mask is not supported (key_padding_mask and is_causal are)')
+    if self.dropout and self.training:
+      raise ValueError('MultiheadAttention: dropout of the probabilities is not supported in training')
+    if self.bias_k is not None or self.bias_v is not None or self.add_zero_attn:
+      raise ValueError('MultiheadAttention: bias_k, bias_v and add_zero_attn are not supported')
+    if query.dim() != 3:
+      raise ValueError('MultiheadAttention: batched inputs only (got %d dimensions)' % query.dim())
+    E = self.embed_dim
+    if self._qkv_same_embed_dim:
+      wq, wk, wv = self.in_proj_weight.split(E)
+    else:
+      wq, wk, wv = self.q_proj_weight, self.k_proj_weight, self.v_proj_weight
+    bq, bk, bv = self.in_proj_bias.split(E) if self.in_proj_bias is not None else (None, None, None)
+    q, k, v = F.linear(query, wq, bq), F.linear(key, wk, bk), F.linear(value, wv, bv)
+    if not self.batch_first:                            # [length, batch, channels]: the heads are views, nothing is moved
+      q, k, v = q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1)
+    heads = [t.unflatten(-1, (self.num_heads, self.head_dim)) for t in (q, k, v)]
+    out = attention(*heads, key_padding_mask=key_padding_mask, is_causal=is_causal).flatten(2)
+    if not self.batch_first:
+      out = out.transpose(0, 1)
+    return self.out_proj(out), None
+
+
+def use_attention_kernels(module):
+  """Switches every torch.nn.MultiheadAttention inside `module` (a TransformerClustering, its `_transformer`, a ViT) over
+  to MultiheadAttention above, in place and without touching its parameters.  Returns how many were switched; a module
+  that could not be called afterwards (dropout, bias_k, add_zero_attn) raises and nothing is switched."""
+  found = [m for m in module.modules() if type(m) is torch.nn.MultiheadAttention]
+  for m in found:
+    if m.dropout or m.bias_k is not None or m.bias_v is not None or m.add_zero_attn:
+      raise ValueError('use_attention_kernels: an attention module uses dropout, bias_k / bias_v or add_zero_attn')
+    if m.head_dim > MAX_HEAD_WIDTH:
+      raise ValueError('use_attention_kernels: head width %d, at most %d' % (m.head_dim, MAX_HEAD_WIDTH))
+  for m in found:
+    m.__class__ = MultiheadAttention
+  return len(found)
 
 
 def forward(self, src, mask, query_embed, pos_embed):

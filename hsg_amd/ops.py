@@ -184,3 +184,120 @@ def normalize_rows(x, eps=EPS):
   if x.dtype != torch.float32:
     raise TypeError('embeddings must be float32')
   return NormalizeRows.apply(x, float(eps))
+
+
+# ---------------------------------------------------------------------------
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _last_contiguous(t):
+  return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _attention_args(q, k, v, padding, causal, scale, out):
+  a = _lib.AttentionArgs()
+  a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+  a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+  if padding is not None and padding.numel():
+    a.padding, a.padding_stride = padding.data_ptr(), padding.stride(0)
+  a.dtype = _TYPE_CODES[q.dtype]
+  a.B, a.L, a.H, a.D = q.shape
+  a.S, a.G = k.shape[1], k.shape[2]
+  a.causal, a.scale = int(causal), float(scale)
+  return a
+
+
+def _attention_call(fn, a, backward, dev):
+  """Runs fn(a) with the workspace it asks for (the caller holds the device guard)."""
+  wsb = _lib.lib().hsgk_attention_workspace_bytes(ctypes.byref(a), backward)
+  ws = torch.empty((wsb,), dtype=torch.uint8, device=dev) if wsb else None
+  if wsb:
+    a.workspace, a.workspace_bytes = ws.data_ptr(), wsb
+  _lib.check(fn(ctypes.byref(a), _lib.stream_ptr()))
+
+
+class Attention(torch.autograd.Function):
+  """hsgk_attention_fwd / _bwd through ctypes (HSGK_BINDING=ctypes; torch_ops.cpp: hsgk::attention)."""
+
+  @staticmethod
+  def forward(ctx, q, k, v, padding, causal, scale):
+    dev = q.device
+    with torch.cuda.device(dev):
+      out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+      a = _attention_args(q, k, v, padding, causal, scale, out)
+      lse = None
+      if any(ctx.needs_input_grad[:3]):
+        lse = torch.empty((a.B, a.G, a.L, a.H // a.G), dtype=torch.float32, device=dev)
+        a.lse = lse.data_ptr()
+      _attention_call(_lib.lib().hsgk_attention_fwd, a, 0, dev)
+    ctx.save_for_backward(q, k, v, padding, out, lse)
+    ctx.cfg = (causal, scale)
+    return out
+
+  @staticmethod
+  def backward(ctx, gout):
+    q, k, v, padding, out, lse = ctx.saved_tensors
+    g = _last_contiguous(gout)
+    dev = q.device
+    want = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+    dk = dv = None
+    with torch.cuda.device(dev):
+      dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+      a = _attention_args(q, k, v, padding, ctx.cfg[0], ctx.cfg[1], out)
+      a.lse, a.dout, a.dq = lse.data_ptr(), g.data_ptr(), dq.data_ptr()
+      a.dout_stride[:] = g.stride()[:3]
+      if want:
+        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
+        a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
+      _attention_call(_lib.lib().hsgk_attention_bwd, a, 1, dev)
+    return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None)
+
+
+def attention(q, k, v, padding, causal, scale):
+  """Checked arguments -> softmax(scale q k^T) v; the public entry (with the argument checks) is
+  models.embeddings.transformer_clusters.attention."""
+  tops = _torch_ops.ops()
+  if tops is not None:                 # the torch-extension binding: one dispatch, C++ autograd node
+    return tops.attention(q, k, v, padding, causal, scale)
+  q, k, v = _last_contiguous(q), _last_contiguous(k), _last_contiguous(v)
+  return Attention.apply(q, k, v, padding if padding is None else _last_contiguous(padding), causal, scale)
+
+
+class TopkDistill(torch.autograd.Function):
+  """hsgk_topk_distill_fwd / _bwd through ctypes (HSGK_BINDING=ctypes; torch_ops.cpp: hsgk::topk_distill)."""
+
+  @staticmethod
+  def forward(ctx, z, teacher, index, temperature):
+    dev = z.device
+    n, V = z.shape
+    with torch.cuda.device(dev):
+      loss = torch.empty((n,), dtype=torch.float32, device=dev)
+      stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+      _lib.check(_lib.lib().hsgk_topk_distill_fwd(
+          z.data_ptr(), _TYPE_CODES[z.dtype], n, V, z.stride(0), teacher.data_ptr(), index.data_ptr(), teacher.shape[1],
+          ctypes.c_float(temperature), loss.data_ptr(), stats.data_ptr() if stats is not None else None,
+          _lib.stream_ptr()))
+    ctx.save_for_backward(z, teacher, index, stats)
+    ctx.temperature = temperature
+    return loss
+
+  @staticmethod
+  def backward(ctx, gloss):
+    z, teacher, index, stats = ctx.saved_tensors
+    n, V = z.shape
+    g = gloss.to(torch.float32).contiguous()
+    with torch.cuda.device(z.device):
+      dz = torch.empty((n, V), dtype=z.dtype, device=z.device)
+      _lib.check(_lib.lib().hsgk_topk_distill_bwd(
+          z.data_ptr(), _TYPE_CODES[z.dtype], n, V, z.stride(0), teacher.data_ptr(), index.data_ptr(), teacher.shape[1],
+          ctypes.c_float(ctx.temperature), stats.data_ptr(), g.data_ptr(), dz.data_ptr(), _lib.stream_ptr()))
+    return dz, None, None, None
+
+
+def topk_distill(z, teacher, index, temperature):
+  """Checked arguments -> per-row loss; the public entry is utils.segsort.loss.topk_distillation_loss."""
+  tops = _torch_ops.ops()
+  if tops is not None:                 # the torch-extension binding: one dispatch, C++ autograd node
+    return tops.topk_distill(z, teacher, index, temperature)
+  return TopkDistill.apply(_last_contiguous(z), teacher.contiguous(), index.contiguous(), temperature)

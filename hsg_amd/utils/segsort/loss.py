@@ -11,6 +11,7 @@ score tiles and contracts them in place (g_emb = W P, g_proto = W^T E) -- no
 [N,P] storage there either.
 """
 import ctypes
+import math
 
 import torch
 from torch.nn.modules.loss import _Loss
@@ -255,3 +256,68 @@ class SetSegSortLoss(_Loss):
     if self.reduction == 'sum':
       return torch.sum(log_likelihood)
     return log_likelihood
+
+
+MAX_TEACHER_ENTRIES = 256      # include/hsgk.h HSGK_DISTILL_MAX_K
+
+
+def topk_distillation_loss(logits, teacher_logits, teacher_indices, temperature=1.0, reduction='mean'):
+  """Distillation of a softmax over the last dimension of `logits` [..., V] (a pixel's similarities to V prototypes) from
+  a teacher of whom only the k best are known: `teacher_logits` and `teacher_indices` [..., k], as
+  `utils.segsort.eval.top_k_indices` returns them (values and indices).
+
+    p = softmax(teacher_logits / T) over the k entries,  q = softmax(logits / T) over all V
+    loss = T^2 sum_j p_j (log p_j - log q_index_j)
+
+  T^2 keeps the gradients' size when T changes.  An entry whose index lies outside [0, V) or whose teacher logit is -inf
+  (an unfilled slot of the retrieval) does not count; a row without any has loss and gradient 0 and still counts as a
+  row of the mean.  An index may come more than once.  logits are float32, bfloat16 or float16, rows at any stride; the
+  loss is float32 ([...] with reduction 'none', else the 'mean' or 'sum' over the rows), the gradient of `logits`'s type.
+  The teacher receives no gradient: teacher_logits that require one are refused."""
+  if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    raise TypeError('logits must be float32, bfloat16 or float16 (got %s)' % logits.dtype)
+  if not teacher_logits.is_floating_point():
+    raise TypeError('teacher_logits must be floating point (got %s)' % teacher_logits.dtype)
+  if teacher_indices.dtype is not torch.int64:
+    raise TypeError('teacher_indices must be int64 (got %s)' % teacher_indices.dtype)
+  if logits.dim() < 1 or logits.shape[-1] < 1:
+    raise ValueError('logits must be [..., V] with V >= 1 (got %s)' % (tuple(logits.shape),))
+  if teacher_logits.shape != teacher_indices.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or \
+      teacher_logits.dim() != logits.dim():
+    raise ValueError('teacher_logits and teacher_indices must be [..., k] with the leading dimensions of logits: %s, %s, %s'
+                     % (tuple(teacher_logits.shape), tuple(teacher_indices.shape), tuple(logits.shape)))
+  if teacher_logits.shape[-1] > MAX_TEACHER_ENTRIES:
+    raise ValueError('at most %d teacher entries a row (got %d)' % (MAX_TEACHER_ENTRIES, teacher_logits.shape[-1]))
+  if teacher_logits.device != logits.device or teacher_indices.device != logits.device:
+    raise ValueError('logits, teacher_logits and teacher_indices must be on one device')
+  if teacher_logits.requires_grad:
+    raise ValueError('teacher_logits must not require a gradient (detach them)')
+  temperature = float(temperature)
+  if not (temperature > 0.0 and math.isfinite(temperature)):
+    raise ValueError('temperature must be positive and finite (got %r)' % temperature)
+  if reduction not in ('none', 'mean', 'sum'):
+    raise ValueError("reduction must be 'none', 'mean' or 'sum' (got %r)" % (reduction,))
+  ops.require_gpu(logits, 'logits')
+  z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+  k = teacher_logits.shape[-1]
+  t = teacher_logits.reshape(z.shape[0], k).to(torch.float32)
+  loss = ops.topk_distill(z, t, teacher_indices.reshape(z.shape[0], k), temperature)
+  if reduction == 'mean':
+    return loss.mean()
+  if reduction == 'sum':
+    return loss.sum()
+  return loss if logits.dim() == 2 else loss.view(logits.shape[:-1])
+
+
+class TopKDistillationLoss(_Loss):
+  """`topk_distillation_loss` as a module beside SegSortLoss."""
+
+  def __init__(self, temperature=1.0, size_average=None, reduce=None, reduction='mean'):
+    super(TopKDistillationLoss, self).__init__(size_average, reduce, reduction)
+    self.temperature = temperature
+
+  def __repr__(self):
+    return 'TopKDistillationLoss(temperature={:.2f})'.format(self.temperature)
+
+  def forward(self, logits, teacher_logits, teacher_indices):
+    return topk_distillation_loss(logits, teacher_logits, teacher_indices, self.temperature, self.reduction)

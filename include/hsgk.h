@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define HSGK_VERSION 401
+#define HSGK_VERSION 402
 #define HSGK_CHUNK 2048          /* rows per segment-sum chunk (order C2)      */
 #define HSGK_EPS 1e-12f          /* normalize_embedding eps (general/common.py:101) */
 
@@ -495,6 +495,54 @@ HSGK_API int hsgk_synth_gaussish(uint64_t key, uint64_t offset, int64_t n, float
 HSGK_API int hsgk_synth_mixture(uint64_t noise_key, uint64_t seed, const float *centres,
                                 int ncentres, int first_image, int B, int C, int H, int W,
                                 float *out, hsgk_stream_t stream);
+
+/* ---- attention: what hsg/models/heads/transformer.py gets from torch.nn.MultiheadAttention between its projections
+ * q, out, dout, dq [B,L,H,D]; k, v, dk, dv [B,S,G,D], H a multiple of G: query head h uses key head h / (H / G).
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that query i sees
+ * A key with padding[b][j] != 0 (padding uint8 [B,S], batch stride padding_stride, nullable) is seen by no query and its
+ * k and v rows may hold anything; with `causal` query i sees the keys j <= i + S - L (the last query sees all).  A query
+ * that sees no key, or only scores of -inf, has output 0 and passes no gradient.
+ * dtype 0 float32, 1 bfloat16, 2 float16; sums, statistics and probabilities are float32, a probability (and its gradient)
+ * is rounded to the 16-bit type where it enters a product of that type.  Strides are in elements: {batch, row, head};
+ * the last dimension is contiguous; out, dq, dk and dv are contiguous and 16-byte aligned.  1 <= D <= 128, scale > 0.
+ * lse float32 [B,G,L,H/G] (forward: nullable; backward: what the forward wrote): log2 of the sum of 2^(score log2 e).
+ * backward: reads out and lse of the forward, recomputes the probabilities, writes dq and (both or neither) dk, dv; no
+ * atomics, the order of every sum is fixed.  The workspace belongs to one call at a time.                            */
+#define HSGK_ATTENTION_MAX_WIDTH 128
+typedef struct hsgk_attention_args {
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const uint8_t *padding;
+  int64_t padding_stride;
+  int32_t dtype, B, L, S, H, G, D, causal;
+  float scale;
+  void *out;
+  float *lse;
+  const void *dout;
+  int64_t dout_stride[3];
+  void *dq, *dk, *dv;
+  void *workspace;
+  size_t workspace_bytes;
+} hsgk_attention_args;
+HSGK_API size_t hsgk_attention_workspace_bytes(const hsgk_attention_args *args, int backward);
+HSGK_API int hsgk_attention_fwd(const hsgk_attention_args *args, hsgk_stream_t stream);
+HSGK_API int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream);
+
+/* ---- distillation from a teacher's k best classes (the prototypes that hsgk_topk_prototypes returns) ----------------
+ * logits [n,V] (dtype 0 float32, 1 bfloat16, 2 float16; rows row_stride elements apart, last dimension contiguous),
+ * teacher float32 [n,k] the teacher's logits of the classes index int64 [n,k].  p = softmax(teacher / T) over the row's
+ * entries, q = softmax(logits / T) over all V:
+ *   loss [n] = T^2 sum_j p_j (log p_j - log q_index_j),  dlogits [n,V] = grad [n] * T (q - sum_j p_j at index_j)
+ * An entry whose index lies outside [0, V) or whose teacher logit is -inf does not count (hsgk_topk_prototypes_grouped
+ * fills with -inf); a row without any has loss 0 and gradient 0.  An index may come more than once.
+ * stats float32 [n,2] (forward: nullable): maximum and sum of exp((logit - maximum) / T), what the backward needs.     */
+#define HSGK_DISTILL_MAX_K 256
+HSGK_API int hsgk_topk_distill_fwd(const void *logits, int dtype, int64_t n, int64_t V, int64_t row_stride,
+                                   const float *teacher, const int64_t *index, int k, float temperature, float *loss,
+                                   float *stats, hsgk_stream_t stream);
+HSGK_API int hsgk_topk_distill_bwd(const void *logits, int dtype, int64_t n, int64_t V, int64_t row_stride,
+                                   const float *teacher, const int64_t *index, int k, float temperature,
+                                   const float *stats, const float *grad, void *dlogits, hsgk_stream_t stream);
 
 #ifdef __cplusplus
 }
