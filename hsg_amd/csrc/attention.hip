@@ -6,30 +6,47 @@
 
 namespace hsgk {
 
+static int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+static int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+
 struct AttnPlan {
-  bool wk;          // 32 columns a workgroup, its waves share the streamed rows (else 128 columns, 32 a wave)
+  bool shared;      // 32 columns a workgroup, its waves share them (else 128, 32 a wave)
   int splits;       // parts of the streamed rows, joined by a second kernel
 };
 
-// Workgroups the plan aims for: two for each of the 256 CUs.
-constexpr int64_t kAttnGroups = 512;
-
-static AttnPlan attn_plan(int64_t heads, int64_t columns, int64_t rows) {
+// Shared columns where 128 of them would leave CUs without a workgroup (float32, 28 heads x 131 queries x 203 keys, width
+// 36: forward 18 us on 126 shared workgroups; 192 heads x 256 x 256, width 32: 29 us on 384 of 128 columns, 40 on 1536
+// shared).  Split rows where there are fewer workgroups than `room`, what the CUs hold at a time: more only add partial
+// results (one token of 16 heads over 2 x 32768 keys, width 128: 256 workgroups 38 + 5 us, 512 42 + 5).  Causal blocks
+// differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys: 1345 us in one part, 773 + 32 in two).
+static AttnPlan attn_plan(const hsgk_attention_args &a, bool dkv) {
+  const int64_t heads = (int64_t)a.B * a.G, queries = (int64_t)a.L * (a.H / a.G);
+  const int64_t columns = dkv ? a.S : queries, rows = dkv ? queries : a.S;
+  const int bytes = padded_width(a.D) * elem_size(a.dtype);                 // of a row in LDS
   AttnPlan p;
-  p.wk = columns <= 32 || heads * ((columns + 127) / 128) < kAttnGroups / 2;
-  const int64_t groups = heads * ((columns + (p.wk ? 31 : 127)) / (p.wk ? 32 : 128));
-  const int64_t tile = p.wk ? 128 : 64;
-  int64_t s = groups > 0 ? (kAttnGroups + groups - 1) / groups : 1;
-  const int64_t most = rows / (2 * tile);
+  p.shared = columns <= 32 || heads * ((columns + 127) / 128) < 256;
+  const int64_t per = p.shared ? 32 : 128, groups = heads * ((columns + per - 1) / per);
+  const bool alone = (p.shared && bytes >= 256) || (dkv && bytes >= 256);   // LDS or registers hold one workgroup a CU
+  const int64_t room = alone && !a.causal ? 256 : 512;
+  int64_t s = groups > 0 ? room / groups : 1;
+  const int64_t most = rows / 256;
   if (s > most) s = most;
+  if (s > kAttnMaxSplits) s = kAttnMaxSplits;
   p.splits = s > 1 ? (int)s : 1;
   return p;
 }
 
-static int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+// whether 16-byte pieces of the rows are aligned
+static bool pieces(const void *p, const int64_t *st, int D, int size) {
+  const int64_t e = 16 / size;
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && D % e == 0 && (!st || (st[0] % e == 0 && st[1] % e == 0 && st[2] % e == 0));
+}
+
+static int loaded_width(const hsgk_attention_args &a) { const int e = 16 / elem_size(a.dtype); return (a.D + e - 1) / e * e; }
 
 struct AttnSpace {
   float *delta, *part, *part2, *ml;
+  void *packed[4];                    // aligned copies of q, k, v, dout where their own rows are not aligned
   size_t bytes;
 };
 
@@ -38,28 +55,29 @@ static AttnSpace attn_space(const hsgk_attention_args &a, bool backward, void *b
   AttnSpace w = {};
   const int64_t heads = (int64_t)a.B * a.G, C = (int64_t)a.L * (a.H / a.G);
   const size_t dp = (size_t)padded_width(a.D);
-  const AttnPlan f = attn_plan(heads, C, a.S);
+  const AttnPlan f = attn_plan(a, false);
   if (!backward) {
     if (f.splits > 1) {
       w.part = c.take<float>((size_t)f.splits * heads * C * dp);
       w.ml = c.take<float>((size_t)f.splits * heads * C * 2);
     }
   } else {
-    const AttnPlan r = attn_plan(heads, a.S, C);
+    const AttnPlan r = attn_plan(a, true);
     const size_t n1 = f.splits > 1 ? (size_t)f.splits * heads * C * dp : 0;
     const size_t n2 = r.splits > 1 ? (size_t)r.splits * heads * a.S * dp : 0;
     w.delta = c.take<float>((size_t)heads * C);
     w.part = c.take<float>(n1 > n2 ? n1 : n2);               // (the two passes follow each other)
     if (n2) w.part2 = c.take<float>(n2);
   }
+  const void *from[4] = {a.q, a.k, a.v, a.dout};
+  const int64_t *st[4] = {a.q_stride, a.k_stride, a.v_stride, a.dout_stride};
+  for (int i = 0; i < (backward ? 4 : 3); ++i)
+    if (!pieces(from[i], st[i], a.D, elem_size(a.dtype))) {
+      const bool query = i == 0 || i == 3;
+      w.packed[i] = c.take<char>((size_t)a.B * (query ? (size_t)a.L * a.H : (size_t)a.S * a.G) * loaded_width(a) * elem_size(a.dtype));
+    }
   w.bytes = c.off;
   return w;
-}
-
-// whether 16-byte pieces of the rows are aligned
-static int pieces(const void *p, const int64_t *st, int D, int size) {
-  const int64_t e = 16 / size;
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && D % e == 0 && (!st || (st[0] % e == 0 && st[1] % e == 0 && st[2] % e == 0));
 }
 
 static int attn_check(const hsgk_attention_args *p, bool backward) {
@@ -82,7 +100,7 @@ static int attn_check(const hsgk_attention_args *p, bool backward) {
     HSGK_REQUIRE(!some || (a.dout && a.lse && a.dq), "null argument");
     HSGK_REQUIRE((!a.dk) == (!a.dv), "dk and dv come together");
   }
-  const int size = a.dtype == 0 ? 4 : 2;
+  const int size = elem_size(a.dtype);
   const uintptr_t all = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                         (backward ? reinterpret_cast<uintptr_t>(a.dout) : 0);
   HSGK_REQUIRE(all % size == 0, "a tensor is not aligned to its elements");
@@ -95,23 +113,52 @@ static int attn_check(const hsgk_attention_args *p, bool backward) {
   return 0;
 }
 
-static AttnArgs attn_args(const hsgk_attention_args &p) {
-  AttnArgs a = {};
-  const int size = p.dtype == 0 ? 4 : 2;
-  a.q = p.q; a.k = p.k; a.v = p.v; a.g = p.dout; a.o = p.out;
-  for (int i = 0; i < 3; ++i) { a.qs[i] = p.q_stride[i]; a.ks[i] = p.k_stride[i]; a.vs[i] = p.v_stride[i]; a.gs[i] = p.dout_stride[i]; }
-  a.pad = p.padding; a.pad_b = p.padding_stride;
-  a.B = p.B; a.L = p.L; a.S = p.S; a.H = p.H; a.G = p.G; a.HG = p.H / p.G; a.D = p.D; a.C = p.L * a.HG;
-  a.causal = p.causal != 0;
-  a.qvec = pieces(a.q, a.qs, a.D, size); a.kvec = pieces(a.k, a.ks, a.D, size); a.vvec = pieces(a.v, a.vs, a.D, size);
-  a.gvec = pieces(a.g, a.gs, a.D, size); a.ovec = pieces(a.o, nullptr, a.D, size);
-  a.scale = p.scale; a.c2 = p.scale * 1.4426950408889634f;
-  a.lse = p.lse;
-  return a;
+template <typename T> static int attn_pack(const void *from, const int64_t *st, int64_t B, int n, int heads, int D, int DL, void *to, hipStream_t s) {
+  const int64_t rows = B * n * heads, blocks = (rows * DL + 255) / 256;
+  if (rows == 0) return 0;
+  hipLaunchKernelGGL(attn_pack_kernel<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, static_cast<const T *>(from),
+                     st[0], st[1], st[2], rows, n, heads, D, DL, static_cast<T *>(to));
+  HSGK_LAUNCH_CHECK();
+  return 0;
 }
 
-static int attn_go(int dtype, AttnPass pass, const AttnArgs &a, bool wk, hipStream_t s) {
-  return dtype == 0 ? attn_f32(pass, a, wk, s) : dtype == 1 ? attn_bf16(pass, a, wk, s) : attn_f16(pass, a, wk, s);
+// the kernels' arguments; copies what they could not read in 16-byte pieces
+static int attn_args(const hsgk_attention_args &p, const AttnSpace &w, bool backward, hipStream_t s, AttnArgs &a) {
+  a = {};
+  const int size = elem_size(p.dtype);
+  a.B = p.B; a.L = p.L; a.S = p.S; a.H = p.H; a.G = p.G; a.HG = p.H / p.G; a.D = p.D; a.C = p.L * a.HG;
+  a.DL = loaded_width(p);
+  const void *from[4] = {p.q, p.k, p.v, p.dout};
+  const int64_t *st[4] = {p.q_stride, p.k_stride, p.v_stride, p.dout_stride};
+  const void **to[4] = {&a.q, &a.k, &a.v, &a.g};
+  int64_t *ts[4] = {a.qs, a.ks, a.vs, a.gs};
+  for (int i = 0; i < (backward ? 4 : 3); ++i) {
+    if (!w.packed[i]) {
+      *to[i] = from[i];
+      for (int x = 0; x < 3; ++x) ts[i][x] = st[i][x];
+      continue;
+    }
+    const bool query = i == 0 || i == 3;
+    const int n = query ? p.L : p.S, heads = query ? p.H : p.G;
+    const int rc = size == 4 ? attn_pack<float>(from[i], st[i], p.B, n, heads, p.D, a.DL, w.packed[i], s)
+                             : attn_pack<_Float16>(from[i], st[i], p.B, n, heads, p.D, a.DL, w.packed[i], s);   // (bits only)
+    if (rc) return rc;
+    *to[i] = w.packed[i];
+    ts[i][0] = (int64_t)n * heads * a.DL; ts[i][1] = (int64_t)heads * a.DL; ts[i][2] = a.DL;
+  }
+  a.o = p.out;
+  a.pad = p.padding; a.pad_b = p.padding_stride;
+  a.causal = p.causal != 0;
+  a.ovec = pieces(a.o, nullptr, a.D, size);
+  a.scale = p.scale; a.c2 = p.scale * 1.4426950408889634f;
+  a.lse = p.lse;
+  return 0;
+}
+
+static int attn_go(int dtype, AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s) {
+  if (pass == kAttnDkv)
+    return dtype == 0 ? attn_dkv_f32(pass, a, shared, s) : dtype == 1 ? attn_dkv_bf16(pass, a, shared, s) : attn_dkv_f16(pass, a, shared, s);
+  return dtype == 0 ? attn_f32(pass, a, shared, s) : dtype == 1 ? attn_bf16(pass, a, shared, s) : attn_f16(pass, a, shared, s);
 }
 
 }  // namespace hsgk
@@ -131,11 +178,13 @@ int hsgk_attention_fwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
   if (int rc = attn_check(args, false)) return rc;
   if ((int64_t)args->B * args->L == 0) return 0;
   (void)hipGetLastError();
-  AttnArgs a = attn_args(*args);
-  const AttnPlan p = attn_plan((int64_t)a.B * a.G, a.C, a.S);
+  hipStream_t s = static_cast<hipStream_t>(stream);
   const AttnSpace w = attn_space(*args, false, args->workspace);
+  AttnArgs a;
+  if (int rc = attn_args(*args, w, false, s, a)) return rc;
+  const AttnPlan p = attn_plan(*args, false);
   a.splits = p.splits; a.part = w.part; a.ml = w.ml; a.out = args->out;
-  return attn_go(args->dtype, kAttnFwd, a, p.wk, static_cast<hipStream_t>(stream));
+  return attn_go(args->dtype, kAttnFwd, a, p.shared, s);
 }
 
 int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
@@ -143,18 +192,19 @@ int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
   if (args->B == 0) return 0;
   (void)hipGetLastError();
   hipStream_t s = static_cast<hipStream_t>(stream);
-  AttnArgs a = attn_args(*args);
   const AttnSpace w = attn_space(*args, true, args->workspace);
+  AttnArgs a;
+  if (int rc = attn_args(*args, w, true, s, a)) return rc;
   a.delta = w.delta; a.part = w.part; a.part2 = w.part2;
   if (a.C > 0) {
-    const AttnPlan p = attn_plan((int64_t)a.B * a.G, a.C, a.S);
+    const AttnPlan p = attn_plan(*args, false);
     a.splits = p.splits; a.out = args->dq;
-    if (int rc = attn_go(args->dtype, kAttnDq, a, p.wk, s)) return rc;
+    if (int rc = attn_go(args->dtype, kAttnDq, a, p.shared, s)) return rc;
   }
   if (a.S > 0 && args->dk) {
-    const AttnPlan p = attn_plan((int64_t)a.B * a.G, a.S, a.C);
+    const AttnPlan p = attn_plan(*args, true);
     a.splits = p.splits; a.out = args->dk; a.out2 = args->dv;
-    if (int rc = attn_go(args->dtype, kAttnDkv, a, p.wk, s)) return rc;
+    if (int rc = attn_go(args->dtype, kAttnDkv, a, p.shared, s)) return rc;
   }
   return 0;
 }

@@ -36,7 +36,8 @@ struct AttnArgs {
   const uint8_t *pad;                    // [B,S], nonzero: not a key (null: all are)
   int64_t pad_b;
   int B, L, S, H, G, HG, D, C;           // HG = H / G, C = L * HG columns per key head
-  int causal, qvec, kvec, vvec, gvec, ovec;   // *vec: 16-byte pieces of that tensor's rows are aligned
+  int DL;                                // D rounded up to 16-byte pieces: what the rows of q, k, v and g hold, aligned
+  int causal, ovec;                      // ovec: 16-byte pieces of the rows of o are aligned
   float scale, c2;
   void *out;                             // o, or dq, or dk (contiguous)
   void *out2;                            // dv
@@ -48,9 +49,24 @@ struct AttnArgs {
 template <typename T> struct Elem;
 template <> struct Elem<float> {
   static constexpr int KS = 8;           // contraction steps of one 16-byte operand pair of lanes
+  static constexpr int MMA = 4;          // matrix instructions that take them
 };
-template <> struct Elem<__bf16> { static constexpr int KS = 16; };
-template <> struct Elem<_Float16> { static constexpr int KS = 16; };
+template <> struct Elem<__bf16> { static constexpr int KS = 16, MMA = 1; };
+template <> struct Elem<_Float16> { static constexpr int KS = 16, MMA = 1; };
+
+// The order of READS LDS reads and MMAS matrix instructions of the code before this line: AHEAD reads first, then in turn,
+// so that an operand is on its way while the matrix unit works on earlier ones (the compiler alone keeps two in flight; dk
+// and dv at width 128, one wave a SIMD: 909 us without, 857 with it; other kernels 0 - 3 %).
+template <int READS, int MMAS, int AHEAD> __device__ __forceinline__ void read_ahead() {
+  constexpr int A = AHEAD < READS ? AHEAD : READS, PER = MMAS / READS;
+  __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+  for (int i = 0; i < READS - A; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, PER, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x8, MMAS - (READS - A) * PER, 0);
+}
 
 __device__ __forceinline__ void mma(f32x16 &acc, const uint4 &a, const uint4 &b, float) {
   const f32x4v x = __builtin_bit_cast(f32x4v, a), y = __builtin_bit_cast(f32x4v, b);
@@ -83,21 +99,6 @@ template <typename T> __device__ __forceinline__ uint4 row_frag(const float (&x)
   }
 }
 
-// 16 bytes of a row from element e0 on, zeros past D
-template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T *row, int e0, int D, bool vec) {
-  constexpr int E = 16 / sizeof(T);
-  if (vec) {                                  // D is a multiple of E: the piece is all inside or all outside
-    return e0 < D ? *reinterpret_cast<const uint4 *>(row + e0) : uint4{0, 0, 0, 0};
-  }
-  T x[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) x[i] = e0 + i < D ? row[e0 + i] : (T)0.0f;
-  uint4 r;
-  __builtin_memcpy(&r, x, 16);
-  return r;
-}
-
 template <typename T> __device__ __forceinline__ float dot_piece(const uint4 &a, const uint4 &b) {
   constexpr int E = 16 / sizeof(T);
   T x[E], y[E];
@@ -109,110 +110,147 @@ template <typename T> __device__ __forceinline__ float dot_piece(const uint4 &a,
   return s;
 }
 
-// workgroup ids are dealt round-robin over the 8 XCDs: consecutive logical ids (the column blocks that stream the same
-// rows) go to ONE XCD and its L2
-__device__ __forceinline__ unsigned xcd_order(unsigned id, unsigned n) {
-  const unsigned x = id & 7, per = n >> 3, rem = n & 7;
-  return x * per + (x < rem ? x : rem) + (id >> 3);
-}
-
+// A tile of streamed rows in LDS, in 16-byte pieces.  Two kinds of reads have to find their data on different banks: 16
+// lanes that take one piece of 16 consecutive rows, and lanes that take 64 bytes of 4 consecutive rows for the transpose
+// (16-bit types; float: 128 bytes of one row).  Piece x of row r lies at x ^ swap(r), which serves both.
 template <typename T, int DP> struct Tile {
-  static constexpr int E = 16 / (int)sizeof(T);          // elements of a 16-byte piece
-  static constexpr int RS = DP + E;                      // LDS row stride: pieces of consecutive rows on different banks
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int E = 16 / (int)sizeof(T);          // elements of a piece
+  static constexpr int PPR = DP / E;                     // pieces per row
   static constexpr int KK = DP / Elem<T>::KS;            // contraction steps over the head width
   static constexpr int RK = 32 / Elem<T>::KS;            // ... over a block of 32 rows
   static constexpr int DB = DP / 32;
-  static constexpr int PPR = DP / E;                     // pieces per row
-  using Columns = uint4[KK];                             // a lane's share of its column vector, as B operands
+  using Columns = uint4[KK];                             // a lane's share of a column vector, as B operands
+  __device__ __forceinline__ static int swap(int r) {    // (depends on r & 15)
+    if constexpr (!kHalf) return DP == 32 ? (r >> 1) & 7 : r & 7;
+    else if constexpr (DP == 32) return (r >> 2) & 3;
+    else if constexpr (DP == 64) return ((r & 2) << 1) | ((r >> 2) & 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+  __device__ __forceinline__ static int piece(int r, int x) { return r * DP + (x ^ swap(r)) * E; }   // element offset
 };
 
-// A operand: 32 consecutive tile rows x contraction step kk over the head width
-template <typename T, int DP>
-__device__ __forceinline__ uint4 frag_rows(const T *tile, int row0, int kk, int lane) {
-  return *reinterpret_cast<const uint4 *>(tile + (row0 + (lane & 31)) * Tile<T, DP>::RS + kk * Elem<T>::KS +
-                                          (lane >> 5) * (Elem<T>::KS / 2));
-}
-
-// A operand of the transposed tile: head elements 32 db .. + 31 x contraction step kk over rows row0 .. row0 + 31
-template <typename T, int DP>
-__device__ __forceinline__ uint4 frag_cols(const T *tile, int row0, int db, int kk, int lane) {
-  constexpr int RS = Tile<T, DP>::RS;
-  if constexpr (sizeof(T) == 4) {
-    const float *p = reinterpret_cast<const float *>(tile) + (row0 + 8 * kk + 4 * (lane >> 5)) * RS + 32 * db + (lane & 31);
-    return __builtin_bit_cast(uint4, f32x4v{p[0], p[RS], p[2 * RS], p[3 * RS]});
-  } else {
-    // 16 lanes hand in the addresses of a 4-row x 16-column patch in 8-byte pieces, lane i of them gets column i
-    const T *p = tile + (row0 + 16 * kk + 4 * (lane >> 5) + ((lane & 15) >> 2)) * RS + 32 * db + 16 * ((lane >> 4) & 1) +
-                 4 * (lane & 3);
-    const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr_h16x4 *)(p));
-    const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr_h16x4 *)(p + 8 * RS));
-    const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
-    return uint4{a.x, a.y, b.x, b.y};
-  }
-}
-
-// streamed rows: registers <- global, LDS <- registers
-template <typename T, int DP, int TR> struct Stage {
-  static constexpr int N = (TR * Tile<T, DP>::PPR + 255) / 256;
-  uint4 r[N];
-  template <typename Row>
-  __device__ __forceinline__ void fetch(Row row_of, int row0, int D, bool vec) {
+// a lane's offsets into a tile: A operands by rows (32 consecutive rows x contraction step over the head width) and by
+// columns (32 head elements x contraction step over 32 rows)
+template <typename T, int DP> struct Lanes {
+  using Ti = Tile<T, DP>;
+  int row[Ti::KK], col[Ti::kHalf ? Ti::DB : 2][Ti::kHalf ? 2 : 4];
+  __device__ __forceinline__ explicit Lanes(int lane) {
+    const int h = lane >> 5;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int id = (int)threadIdx.x + 256 * n;
-      const int row = id / Tile<T, DP>::PPR, e0 = (id % Tile<T, DP>::PPR) * Tile<T, DP>::E;
-      r[n] = uint4{0, 0, 0, 0};
-      if (row < TR) {
-        const T *p = row_of(row0 + row);
-        if (p) r[n] = load_piece<T>(p, e0, D, vec);
-      }
+    for (int kk = 0; kk < Ti::KK; ++kk) row[kk] = Ti::piece(lane & 31, 2 * kk + h);
+    if constexpr (Ti::kHalf) {
+      // 16 lanes hand in the addresses of a 4-row x 16-column patch in 8-byte pieces, lane i of them gets column i
+      const int r = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+      for (int db = 0; db < Ti::DB; ++db)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          col[db][u] = Ti::piece(r + 8 * u, 4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 4 * (lane & 1);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) col[u][i] = Ti::piece(8 * u + 4 * h + i, (lane & 31) >> 2) + (lane & 3) - 8 * u * DP;
     }
   }
-  __device__ __forceinline__ void store(T *tile) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int id = (int)threadIdx.x + 256 * n;
-      const int row = id / Tile<T, DP>::PPR, e0 = (id % Tile<T, DP>::PPR) * Tile<T, DP>::E;
-      if (row < TR) *reinterpret_cast<uint4 *>(tile + row * Tile<T, DP>::RS + e0) = r[n];
+  __device__ __forceinline__ uint4 rows(const T *tile, int row0, int kk) const {
+    return *reinterpret_cast<const uint4 *>(tile + row0 * DP + row[kk]);
+  }
+  __device__ __forceinline__ uint4 cols(const T *tile, int row0, int db, int kk) const {
+    if constexpr (Ti::kHalf) {
+      const T *p = tile + (row0 + 16 * kk) * DP;
+      const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr_h16x4 *)(p + col[db][0]));
+      const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr_h16x4 *)(p + col[db][1]));
+      const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+      return uint4{a.x, a.y, b.x, b.y};
+    } else {
+      const float *p = reinterpret_cast<const float *>(tile) + (row0 + 8 * kk) * DP + 32 * db;
+      const int *c = col[kk & 1];
+      return __builtin_bit_cast(uint4, f32x4v{p[c[0]], p[c[1]], p[c[2]], p[c[3]]});
     }
   }
 };
 
-// column vectors of the lane, kept as B operands
-template <typename T, int DP>
-__device__ __forceinline__ void load_columns(typename Tile<T, DP>::Columns &x, const T *row, int D, bool vec, int lane) {
+// keeps a rarely taken branch a branch: the compiler would compute both sides of every element
+__device__ __forceinline__ void rare() { asm volatile("; rare"); }
+
+// Streamed rows go from memory straight into LDS, 16 bytes a lane (a wave fills 1 KB in lane order, so a lane fetches the
+// piece that belongs into its place); no register holds them on the way.  Written as an instruction because the compiler
+// would wait for it at the next LDS read, whichever buffer that reads; the loop waits itself (stream()).
+__device__ __forceinline__ void load_to_lds(const void *from, uint32_t lds_byte) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_byte), "v"(from) : "memory");
+}
+// (the builtin, not an instruction of ours: the compiler then knows that its own loads from before the loop have arrived and
+//  does not wait for them -- and so for the tile under way -- at their first use inside it)
+__device__ __forceinline__ void wait_for_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)(p);
+}
+
+template <typename T, int DP, int TR> struct Rows {
+  using Ti = Tile<T, DP>;
+  static constexpr int N = TR * Ti::PPR / 256;
+  static_assert(TR * Ti::PPR % 256 == 0, "a tile is a whole number of pieces a thread");
+  const T *p[N];
+  __device__ __forceinline__ static int row_of(int n) { return ((int)threadIdx.x + 256 * n) / Ti::PPR; }
+  __device__ __forceinline__ static int piece_of(int n) {
+    return (((int)threadIdx.x + 256 * n) % Ti::PPR) ^ Ti::swap(row_of(n) & 15);
+  }
+  // a row at or past `end` is fetched as row end - 1: its scores are hidden, and what it holds enters other sums already
+  template <typename At> __device__ __forceinline__ void place(At at, int row0, int end) {
 #pragma unroll
-  for (int kk = 0; kk < Tile<T, DP>::KK; ++kk)
-    x[kk] = row ? load_piece<T>(row, kk * Elem<T>::KS + (lane >> 5) * (Elem<T>::KS / 2), D, vec) : uint4{0, 0, 0, 0};
+    for (int n = 0; n < N; ++n) p[n] = at(min(row0 + row_of(n), end - 1)) + piece_of(n) * Ti::E;
+  }
+  __device__ __forceinline__ void advance(int64_t by) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) p[n] += by;
+  }
+  // D: elements of a row rounded up to pieces; the places behind it were zeroed once
+  __device__ __forceinline__ void issue(const T *tile, int D) const {
+    const uint32_t base = lds_address(tile) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (piece_of(n) * Ti::E < D) load_to_lds(p[n], base + n * 4096);
+  }
+  // bit n of gone: piece n belongs to a row that nobody sees; it may hold anything and becomes zero
+  __device__ __forceinline__ static void clear(T *tile, uint32_t gone) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if ((gone >> n) & 1) *reinterpret_cast<uint4 *>(tile + ((int)threadIdx.x + 256 * n) * Ti::E) = uint4{0, 0, 0, 0};
+  }
+};
+
+// 16 bytes of a row from element e0 on, zeros past D
+template <typename T> __device__ __forceinline__ uint4 load_piece(const T *row, int e0, int D, bool vec) {
+  constexpr int E = 16 / sizeof(T);
+  if (vec) return e0 < D ? *reinterpret_cast<const uint4 *>(row + e0) : uint4{0, 0, 0, 0};
+  T x[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) x[i] = e0 + i < D ? row[e0 + i] : (T)0.0f;
+  uint4 r;
+  __builtin_memcpy(&r, x, 16);
+  return r;
+}
+
+// column vectors of the lane, kept as B operands (D: rounded up to pieces)
+template <typename T, int DP>
+__device__ __forceinline__ void load_columns(typename Tile<T, DP>::Columns &x, const T *row, int D, int lane) {
+#pragma unroll
+  for (int kk = 0; kk < Tile<T, DP>::KK; ++kk) {
+    const int e0 = kk * Elem<T>::KS + (lane >> 5) * (Elem<T>::KS / 2);
+    x[kk] = row && e0 < D ? *reinterpret_cast<const uint4 *>(row + e0) : uint4{0, 0, 0, 0};
+  }
 }
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
 __device__ __forceinline__ void col_of(const AttnArgs &a, int c, int &i, int &hh) {
   if (a.HG == 1) { i = c; hh = 0; } else { i = (int)((unsigned)c / (unsigned)a.HG); hh = c - i * a.HG; }
-}
-
-// first and last + 1 visible key of [lo, hi) (workgroup-uniform); hi <= lo when there is none
-__device__ inline void visible_range(const uint8_t *pad, int &lo, int &hi, int *red) {
-  int first = hi, last = lo;
-  for (int j = lo + (int)threadIdx.x; j < hi; j += 256)
-    if (!pad[j]) { first = j < first ? j : first; last = j + 1; }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const int f = __shfl_xor(first, off), l = __shfl_xor(last, off);
-    first = f < first ? f : first;
-    last = l > last ? l : last;
-  }
-  if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = first; red[4 + (threadIdx.x >> 6)] = last; }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    first = red[w] < first ? red[w] : first;
-    last = red[4 + w] > last ? red[4 + w] : last;
-  }
-  __syncthreads();
-  lo = first;
-  hi = last;
 }
 
 template <typename T> __device__ __forceinline__ void store4(T *p, float a, float b, float c, float d) {
@@ -249,14 +287,11 @@ template <typename T, int DB> struct ColumnScale {
   __device__ __forceinline__ void start() {
     if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) f = 0x1p100f;
   }
-  template <int NS>
-  __device__ __forceinline__ void apply(float (&ds)[NS][16], f32x16 (&acc)[DB]) {
+  __device__ __forceinline__ void apply(float (&ds)[16], f32x16 (&acc)[DB]) {
     if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
       float top = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[n][r]));
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
       top = fmaxf(top, other_half(top));
       if (__any(top * f > 32768.0f)) {
         if (top * f > 32768.0f) {
@@ -273,9 +308,7 @@ template <typename T, int DB> struct ColumnScale {
         }
       }
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ds[n][r] *= f;
+      for (int r = 0; r < 16; ++r) ds[r] *= f;
     }
   }
 };
@@ -284,18 +317,27 @@ template <typename T> constexpr float prob_shift() {         // log2 of the fact
   return sizeof(T) == 2 && !__is_same(T, __bf16) ? 15.0f : 0.0f;
 }
 
-template <typename T, int DP, bool WK> struct Shape {
-  static constexpr int TR = WK ? 128 : (sizeof(T) == 4 && DP == 128 ? 32 : 64);   // streamed rows per tile
-  static constexpr int NS = WK ? TR / 128 : TR / 32;                               // 32-row blocks of a wave per tile
-  static constexpr int COLS = WK ? 32 : 128;                                       // columns of a workgroup
-  static constexpr int TILE = TR * Tile<T, DP>::RS * (int)sizeof(T);               // bytes of one staged tile
-  static constexpr int NBUF = 4 * TILE <= 80 * 1024 ? 2 : 1;
-  static constexpr int JOIN = WK ? 4 * 32 * (DP + 1) * 4 : 0;
+// A workgroup of four waves with 32 columns each (KW = 1), or with the same 32 columns, each wave on a quarter of every
+// tile's rows, their results joined at the end (KW = 4: few columns).
+// (Measured and not kept: 64 columns a wave, so that an A operand read from LDS serves two matrix instructions.  bfloat16,
+// us for 32, 64 and 2 x 64 columns with halved rows: forward of 16 heads x 8192 x 8192 causal, width 128, 435, 680, 901;
+// 96 heads x 785 x 785, width 64, 37, 46, 71.  One wave less a SIMD costs more than the LDS traffic.)
+template <typename T, int DP, int KW> struct Shape {
+  static constexpr int COLS = 128 / KW;                                            // columns of a workgroup
+  static constexpr int TR = KW == 4 ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64; // streamed rows per tile
+  static constexpr int NS = TR / KW / 32;                                          // 32-row blocks of a wave per tile
+  static constexpr int TILE = TR * DP * (int)sizeof(T);                            // bytes of one staged tile
+  static constexpr int NBUF = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int JOIN = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
   static constexpr int LDS = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  static constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;                                            // see read_ahead
+  // waves of a SIMD that the registers have to leave room for (no more than the LDS does)
+  static constexpr int W0 = LDS > 80 * 1024 ? 1 : LDS > 52 * 1024 ? 2 : 3;
+  static constexpr int WF = DP == 32 ? W0 : W0 < 2 || (sizeof(T) == 4 && DP == 128) ? 1 : 2;
+  static constexpr int WB = DP == 128 ? 1 : WF;
 };
 
-// the four waves' partial results of the same 32 columns: acc * f summed over the waves in wave order
-// (the caller has synchronised: the tiles are no longer read)
+// partial results of the waves, for the join (the caller synchronises before and after)
 template <int DP>
 __device__ __forceinline__ void join_put(float *lds, const f32x16 (&acc)[DP / 32], float f, int w, int lane) {
   float *p = lds + (w * 32 + (lane & 31)) * (DP + 1) + 4 * (lane >> 5);
@@ -304,108 +346,223 @@ __device__ __forceinline__ void join_put(float *lds, const f32x16 (&acc)[DP / 32
 #pragma unroll
     for (int r = 0; r < 16; ++r) p[32 * db + 8 * (r >> 2) + (r & 3)] = acc[db][r] * f;
 }
+// element d of column col: the sum over the waves, in wave order
 template <int DP> __device__ __forceinline__ float join_get(const float *lds, int col, int d) {
   const float *p = lds + col * (DP + 1) + d;
   return ((p[0] + p[32 * (DP + 1)]) + p[2 * 32 * (DP + 1)]) + p[3 * 32 * (DP + 1)];
 }
 
+// the tiles of [lo, hi), the first of which is on its way (issue(lo, 0)): the next one is while one is computed on.
+// land(buf): what a thread still does to its own share of the tile that has arrived, before the others see it.
+template <int TR, int NBUF, typename Issue, typename Land, typename Compute>
+__device__ __forceinline__ void stream(int lo, int hi, Issue issue, Land land, Compute compute) {
+  int buf = 0;
+  for (int t0 = lo; t0 < hi; t0 += TR) {
+    const bool more = t0 + TR < hi;
+    wait_for_lds();
+    land(buf);
+    __syncthreads();                          // the tile is whole, and nobody reads the other buffer any more
+    if (NBUF == 2 && more) issue(t0 + TR, buf ^ 1);
+    compute(t0, buf);
+    if (NBUF == 2) {
+      buf ^= 1;
+    } else if (more) {
+      __syncthreads();
+      issue(t0 + TR, 0);
+    }
+  }
+  wait_for_lds();                             // (the first tile of an empty range)
+}
+
+// zeros where the tiles' rows end before DP
+template <int BYTES> __device__ __forceinline__ void clear_tiles(unsigned char *lds, bool narrow) {
+  if (!narrow) return;
+  for (int t = (int)threadIdx.x * 16; t < BYTES; t += 256 * 16) *reinterpret_cast<uint4 *>(lds + t) = uint4{0, 0, 0, 0};
+  __syncthreads();
+}
+
+// Which part, column block and (batch item, key head) a workgroup takes.  Workgroup ids are dealt round-robin over the 8
+// XCDs, each with an L2 of its own: workgroups that stream the same rows belong on one XCD.  Without causality consecutive
+// blocks of a head go to the same XCD; with it the blocks differ in work, so the longest of all heads come first and the
+// heads take turns (with 8 heads or a divisor or multiple of 8 a head still stays on its XCDs).  Parts of split rows are
+// counted from the end that every block sees, so the first parts are whole, and neighbours in the order differ little: within
+// an XCD workgroups are placed in order, and one that has to wait holds up the rest (dk and dv of 16 heads on 4, 8192 x 8192,
+// width 128: 1318 us with the two parts of a block next to each other, 857 this way).
+struct Place {
+  int sp, cb, bg;
+};
+__device__ __forceinline__ Place place_of(const AttnArgs &a, int blocks, bool descending) {
+  Place p;
+  unsigned id = blockIdx.x;
+  if (a.causal) {
+    const unsigned heads = (unsigned)(a.B * a.G);
+    p.bg = (int)(id % heads);
+    id /= heads;
+    p.sp = (int)(id / (unsigned)blocks);
+    p.cb = (int)(id % (unsigned)blocks);
+    if (descending) p.cb = blocks - 1 - p.cb;
+  } else {
+    const unsigned n = gridDim.x, x = id & 7, per = n >> 3, rem = n & 7;
+    id = x * per + (x < rem ? x : rem) + (id >> 3);
+    p.sp = (int)(id % (unsigned)a.splits);
+    id /= (unsigned)a.splits;
+    p.cb = (int)(id % (unsigned)blocks);
+    p.bg = (int)(id / (unsigned)blocks);
+  }
+  return p;
+}
+
+// the keys [lo, hi) of a workgroup with columns c0 .. c0 + cols - 1: its split, what its last query sees; first_limit: the
+// last key that its first query sees
+__device__ __forceinline__ void key_range(const AttnArgs &a, int sp, int tr, int c0, int cols, int &lo, int &hi, int &first_limit) {
+  lo = 0; hi = a.S; first_limit = a.S;
+  if (a.splits > 1) {
+    const int chunk = ((a.S + a.splits - 1) / a.splits + tr - 1) / tr * tr;
+    lo = (int)min((int64_t)sp * chunk, (int64_t)a.S);
+    hi = min(lo + chunk, a.S);
+  }
+  if (a.causal) {
+    int il, ih;
+    col_of(a, min(c0 + cols, a.C) - 1, il, ih);
+    hi = min(hi, il + a.S - a.L + 1);
+    col_of(a, c0, il, ih);
+    first_limit = il + a.S - a.L;
+  }
+}
+
+// last + 1 visible key of [lo, hi) (workgroup-uniform; lo when there is none)
+__device__ inline int visible_end(const uint8_t *pad, int lo, int hi, int *red) {
+  int last = lo;
+  for (int j = lo + (int)threadIdx.x; j < hi; j += 256)
+    if (!pad[j]) last = j + 1;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const int l = __shfl_xor(last, off);
+    last = l > last ? l : last;
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = last;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) last = red[w] > last ? red[w] : last;
+  return __builtin_amdgcn_readfirstlane(last);
+}
+
+// keys and values of one (batch item, key head) on their way into LDS, with the flags of the keys that nobody sees
+template <typename T, int DP, int TR> struct KeyRows {
+  Rows<T, DP, TR> k, v;
+  const T *kb, *vb;
+  uint32_t gone = 0;
+  int hidden = 0;
+  __device__ __forceinline__ void issue(const AttnArgs &a, const uint8_t *pad, int lo, int t0, int hi, const T *tk, const T *tv) {
+    if (t0 == lo || t0 + TR > hi) {
+      k.place([&](int j) { return kb + (int64_t)j * a.ks[1]; }, t0, hi);
+      v.place([&](int j) { return vb + (int64_t)j * a.vs[1]; }, t0, hi);
+    } else {
+      k.advance((int64_t)TR * a.ks[1]);
+      v.advance((int64_t)TR * a.vs[1]);
+    }
+    k.issue(tk, a.DL);
+    v.issue(tv, a.DL);
+    const int j = t0 + (int)threadIdx.x;
+    hidden = j >= hi;
+    if (pad) {
+      gone = 0;
+#pragma unroll
+      for (int n = 0; n < Rows<T, DP, TR>::N; ++n) {
+        const int jn = t0 + Rows<T, DP, TR>::row_of(n);
+        if (jn >= hi || pad[jn]) gone |= 1u << n;   // (behind the end comes row end - 1, which may be padded)
+      }
+      if ((int)threadIdx.x < TR && j < hi) hidden = pad[j];
+    }
+  }
+  __device__ __forceinline__ void land(T *tk, T *tv, int *hid) const {
+    if (gone) {
+      Rows<T, DP, TR>::clear(tk, gone);
+      Rows<T, DP, TR>::clear(tv, gone);
+    }
+    if ((int)threadIdx.x < TR) hid[threadIdx.x] = hidden;
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------------------------
-// forward.  WK = false: four waves, 128 columns, every wave walks all keys; WK = true: 32 columns, each wave takes a
-// quarter of every tile's keys and the four results are joined (few columns)
-template <typename T, int DP, bool WK> __global__ __launch_bounds__(256) void attn_fwd_kernel(const AttnArgs a) {
-  using Sh = Shape<T, DP, WK>;
+// forward: columns = queries, keys and values stream
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))
+void attn_fwd_kernel(const AttnArgs a) {
+  using Sh = Shape<T, DP, KW>;
   using Ti = Tile<T, DP>;
   constexpr int TR = Sh::TR, NS = Sh::NS;
   __shared__ __attribute__((aligned(16))) unsigned char lds[Sh::LDS];
   __shared__ __attribute__((aligned(16))) int hid[Sh::NBUF][TR];
   __shared__ float stat[2][4][32];
+  __shared__ int red[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-  const int ncb = (a.C + Sh::COLS - 1) / Sh::COLS;
-  unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int sp = (int)(id % (unsigned)a.splits);
-  id /= (unsigned)a.splits;
-  int cb = (int)(id % (unsigned)ncb);
-  const int bg = (int)(id / (unsigned)ncb), b = bg / a.G, gh = bg - b * a.G;
-  if (a.causal) cb = ncb - 1 - cb;                                    // the longest first
-  const int c0 = cb * Sh::COLS, c = c0 + (WK ? 0 : 32 * w) + (lane & 31);
-  const bool mine = c < a.C;
-  int i, hh;
-  col_of(a, mine ? c : 0, i, hh);
-  const T *kb = static_cast<const T *>(a.k) + (int64_t)b * a.ks[0] + (int64_t)gh * a.ks[2];
-  const T *vb = static_cast<const T *>(a.v) + (int64_t)b * a.vs[0] + (int64_t)gh * a.vs[2];
+  const Place at = place_of(a, (a.C + Sh::COLS - 1) / Sh::COLS, true);
+  const int b = at.bg / a.G, gh = at.bg - b * a.G;
+  const int c0 = at.cb * Sh::COLS, c = c0 + (KW == 1 ? 32 * w : 0) + (lane & 31);
   const uint8_t *pad = a.pad ? a.pad + (int64_t)b * a.pad_b : nullptr;
-  uint4 q[Ti::KK];
-  load_columns<T, DP>(q, mine ? static_cast<const T *>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] +
-                                    (int64_t)(gh * a.HG + hh) * a.qs[2]
-                              : nullptr, a.D, a.qvec, lane);
-  // keys of this workgroup
-  int lo = 0, hi = a.S, first_limit = a.S;
-  if (a.splits > 1) {
-    const int chunk = ((a.S + a.splits - 1) / a.splits + TR - 1) / TR * TR;
-    lo = (int)min((int64_t)sp * chunk, (int64_t)a.S);
-    hi = min(lo + chunk, a.S);
-  }
+  int lo, hi, first_limit;
+  key_range(a, at.sp, TR, c0, Sh::COLS, lo, hi, first_limit);
+  auto tile = [&](int buf, int which) { return reinterpret_cast<T *>(lds + (2 * buf + which) * Sh::TILE); };
+  clear_tiles<2 * Sh::NBUF * Sh::TILE>(lds, a.DL < DP);
+  KeyRows<T, DP, TR> st;
+  st.kb = static_cast<const T *>(a.k) + (int64_t)b * a.ks[0] + (int64_t)gh * a.ks[2];
+  st.vb = static_cast<const T *>(a.v) + (int64_t)b * a.vs[0] + (int64_t)gh * a.vs[2];
+  auto issue = [&](int t0, int buf) { st.issue(a, pad, lo, t0, hi, tile(buf, 0), tile(buf, 1)); };
+  if (lo < hi) issue(lo, 0);
+
+  const Lanes<T, DP> ln(lane);
+  typename Ti::Columns q;
+  int i, hh;
+  col_of(a, c < a.C ? c : 0, i, hh);
+  load_columns<T, DP>(q, c < a.C ? static_cast<const T *>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] +
+                                       (int64_t)(gh * a.HG + hh) * a.qs[2]
+                                 : nullptr, a.DL, lane);
   const int lim = a.causal ? i + a.S - a.L : a.S;                     // the last key that the column sees
-  if (a.causal) {
-    int il, ih;
-    col_of(a, min(c0 + Sh::COLS, a.C) - 1, il, ih);
-    hi = min(hi, il + a.S - a.L + 1);
-    col_of(a, c0, il, ih);
-    first_limit = il + a.S - a.L;
-  }
-  if (pad && lo < hi) visible_range(pad, lo, hi, reinterpret_cast<int *>(&stat[0][0][0]));
+  if (pad && lo < hi) hi = visible_end(pad, lo, hi, red);
 
   f32x16 acc[Ti::DB];
 #pragma unroll
   for (int db = 0; db < Ti::DB; ++db) acc[db] = f32x16{0.0f};
   float m = -__builtin_inff(), l = 0.0f;                              // maximum of the scores, this half's sum
-  Stage<T, DP, TR> sk, sv;
-  int hidden = 0;
-  auto fetch = [&](int t0) {
-    // (a row behind the last key is not read; a padded one is read and replaced by zeros, whatever it holds)
-    sk.fetch([&](int j) -> const T * { return j < hi && !(pad && pad[j]) ? kb + (int64_t)j * a.ks[1] : nullptr; }, t0, a.D, a.kvec);
-    sv.fetch([&](int j) -> const T * { return j < hi && !(pad && pad[j]) ? vb + (int64_t)j * a.vs[1] : nullptr; }, t0, a.D, a.vvec);
-    if ((int)threadIdx.x < TR) hidden = t0 + (int)threadIdx.x >= hi || (pad && pad[t0 + (int)threadIdx.x]);
-  };
-  auto put = [&](int buf) {
-    sk.store(reinterpret_cast<T *>(lds + (2 * buf) * Sh::TILE));
-    sv.store(reinterpret_cast<T *>(lds + (2 * buf + 1) * Sh::TILE));
-    if ((int)threadIdx.x < TR) hid[buf][threadIdx.x] = hidden;
-  };
   auto compute = [&](int t0, int buf) {
-    const T *tk = reinterpret_cast<const T *>(lds + (2 * buf) * Sh::TILE);
-    const T *tv = reinterpret_cast<const T *>(lds + (2 * buf + 1) * Sh::TILE);
-    const int r0 = WK ? 32 * NS * w : 0;
+    const T *tk = tile(buf, 0), *tv = tile(buf, 1);
+    const int r0 = KW == 1 ? 0 : 32 * NS * w;
     float s[NS][16];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      f32x16 x = f32x16{0.0f};
+    for (int x = 0; x < NS; ++x) {
+      f32x16 y = f32x16{0.0f};
 #pragma unroll
-      for (int kk = 0; kk < Ti::KK; ++kk) mma(x, frag_rows<T, DP>(tk, r0 + 32 * n, kk, lane), q[kk], T());
+      for (int kk = 0; kk < Ti::KK; ++kk) mma(y, ln.rows(tk, r0 + 32 * x, kk), q[kk], T());
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[n][r] = x[r];
+      for (int r = 0; r < 16; ++r) s[x][r] = y[r];
     }
-    if (pad || t0 + TR > hi || t0 + TR - 1 > first_limit) {
+    read_ahead<NS * Ti::KK, NS * Ti::KK * Elem<T>::MMA, Sh::AHEAD>();
+    uint4 fv[Ti::DB];
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
+    for (int db = 0; db < Ti::DB; ++db) fv[db] = ln.cols(tv, r0, db, 0);
+    if (pad || t0 + TR > hi || t0 + TR - 1 > first_limit) {
+      rare();
+#pragma unroll
+      for (int x = 0; x < NS; ++x)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int row = r0 + 32 * n + 8 * r4 + 4 * h;
-          const int4 hd = *reinterpret_cast<const int4 *>(&hid[buf][row]);
-          const int hx[4] = {hd.x, hd.y, hd.z, hd.w};
+          const int row = r0 + 32 * x + 8 * r4 + 4 * h;
+          const int4 hv = *reinterpret_cast<const int4 *>(&hid[buf][row]);
+          const int hx[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (hx[e] || t0 + row + e > lim) s[n][4 * r4 + e] = -__builtin_inff();
+            if (hx[e] || t0 + row + e > lim) s[x][4 * r4 + e] = -__builtin_inff();
         }
     }
     float top = s[0][0];
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int x = 0; x < NS; ++x)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[n][r]);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[x][r]);
     top = fmaxf(top, other_half(top));
     const float mn = fmaxf(m, top);
-    if (__any(mn > m)) {                                              // (rows whose maximum stays: factor 1)
+    if (__any(mn > m)) {                                              // (a column whose maximum stays: factor 1)
       const float f = mn > m ? exp2f((m - mn) * a.c2) : 1.0f;
       l *= f;
 #pragma unroll
@@ -416,106 +573,101 @@ template <typename T, int DP, bool WK> __global__ __launch_bounds__(256) void at
     }
     const float base = m == -__builtin_inff() ? 0.0f : prob_shift<T>() - m * a.c2;
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int x = 0; x < NS; ++x)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.c2, base));
-        l += s[n][r];
+        s[x][r] = __builtin_amdgcn_exp2f(fmaf(s[x][r], a.c2, base));
+        l += s[x][r];
       }
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int x = 0; x < NS; ++x)
 #pragma unroll
       for (int kk = 0; kk < Ti::RK; ++kk) {
-        const uint4 p = row_frag<T>(s[n], kk);
+        const uint4 p = row_frag<T>(s[x], kk);
+        const int next = x * Ti::RK + kk + 1;
 #pragma unroll
-        for (int db = 0; db < Ti::DB; ++db) mma(acc[db], frag_cols<T, DP>(tv, r0 + 32 * n, db, kk, lane), p, T());
+        for (int db = 0; db < Ti::DB; ++db) {
+          mma(acc[db], fv[db], p, T());
+          if (next < NS * Ti::RK) fv[db] = ln.cols(tv, r0 + 32 * (next / Ti::RK), db, next % Ti::RK);
+        }
       }
   };
+  stream<TR, Sh::NBUF>(lo, hi, issue, [&](int buf) { st.land(tile(buf, 0), tile(buf, 1), hid[buf]); }, compute);
 
-  if (lo < hi) {
-    fetch(lo);
-    if (Sh::NBUF == 2) put(0);
-    int buf = 0;
-    for (int t0 = lo; t0 < hi; t0 += TR) {
-      const bool more = t0 + TR < hi;
-      if (Sh::NBUF == 2) {
-        if (more) fetch(t0 + TR);
-        __syncthreads();
-        compute(t0, buf);
-        if (more) put(buf ^ 1);
-        buf ^= 1;
-      } else {
-        __syncthreads();
-        put(0);
-        __syncthreads();
-        if (more) fetch(t0 + TR);
-        compute(t0, 0);
-      }
-    }
-  }
   l += other_half(l);
-  const int64_t at = (int64_t)bg * a.C + c;
-  const int64_t prow = (int64_t)sp * a.B * a.G * a.C + at;
-  T *orow = static_cast<T *>(a.out) + (((int64_t)b * a.L + i) * a.H + gh * a.HG + hh) * a.D;
-  float mt = m * a.c2 - prob_shift<T>();                              // log2 of the factor taken out of l and acc
-  if (l == 0.0f) mt = -__builtin_inff();
-  if constexpr (WK) {
+  const float mt = l == 0.0f ? -__builtin_inff() : m * a.c2 - prob_shift<T>();       // log2 of the factor taken out of l and acc
+  auto out_row = [&](int ci, int ch) { return static_cast<T *>(a.out) + (((int64_t)b * a.L + ci) * a.H + gh * a.HG + ch) * a.D; };
+  const int64_t first = (int64_t)at.bg * a.C, part = (int64_t)at.sp * a.B * a.G * a.C;
+  if constexpr (KW > 1) {
+    float *jo = reinterpret_cast<float *>(lds);
     __syncthreads();
     if (h == 0) { stat[0][w][lane] = mt; stat[1][w][lane] = l; }
     __syncthreads();
-    const int cl = lane & 31;
-    float M = fmaxf(fmaxf(stat[0][0][cl], stat[0][1][cl]), fmaxf(stat[0][2][cl], stat[0][3][cl]));
-    if (M == -__builtin_inff()) M = 0.0f;
-    join_put<DP>(reinterpret_cast<float *>(lds), acc, exp2f(mt - M), w, lane);
+    auto top = [&](int col) { return fmaxf(fmaxf(stat[0][0][col], stat[0][1][col]), fmaxf(stat[0][2][col], stat[0][3][col])); };
+    const float M = top(lane & 31);
+    join_put<DP>(jo, acc, exp2f(mt - (M == -__builtin_inff() ? 0.0f : M)), w, lane);
     __syncthreads();
     for (int t = threadIdx.x; t < 32 * DP; t += 256) {
       const int col = t / DP, d = t % DP, cc = c0 + col;
       if (cc >= a.C) continue;
-      float MM = fmaxf(fmaxf(stat[0][0][col], stat[0][1][col]), fmaxf(stat[0][2][col], stat[0][3][col]));
+      float MM = top(col), L = 0.0f;
       const bool none = MM == -__builtin_inff();
       if (none) MM = 0.0f;
-      float L = 0.0f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) L += stat[1][x][col] * exp2f(stat[0][x][col] - MM);
-      const float o = join_get<DP>(reinterpret_cast<const float *>(lds), col, d);
-      const int64_t ac = (int64_t)bg * a.C + cc, pc = (int64_t)sp * a.B * a.G * a.C + ac;
+      for (int k = 0; k < KW; ++k) L += stat[1][k][col] * exp2f(stat[0][k][col] - MM);
+      const float o = join_get<DP>(jo, col, d);
       if (a.splits > 1) {
-        a.part[pc * DP + d] = o;
-        if (d == 0) { a.ml[2 * pc] = none ? -__builtin_inff() : MM; a.ml[2 * pc + 1] = L; }
+        a.part[(part + first + cc) * DP + d] = o;
+        if (d == 0) { a.ml[2 * (part + first + cc)] = none ? -__builtin_inff() : MM; a.ml[2 * (part + first + cc) + 1] = L; }
       } else {
         int ci, ch;
         col_of(a, cc, ci, ch);
-        if (d < a.D)
-          static_cast<T *>(a.out)[(((int64_t)b * a.L + ci) * a.H + gh * a.HG + ch) * a.D + d] = (T)(L == 0.0f ? 0.0f : o / L);
-        if (d == 0 && a.lse) a.lse[ac] = L == 0.0f ? __builtin_inff() : MM + log2f(L);
+        if (d < a.D) out_row(ci, ch)[d] = (T)(L == 0.0f ? 0.0f : o / L);
+        if (d == 0 && a.lse) a.lse[first + cc] = L == 0.0f ? __builtin_inff() : MM + log2f(L);
       }
     }
-  } else if (mine) {
+  } else if (c < a.C) {
     if (a.splits > 1) {
-      store_column<float, Ti::DB>(a.part + prow * DP, acc, 1.0f, DP, lane);
-      if (h == 0) { a.ml[2 * prow] = mt; a.ml[2 * prow + 1] = l; }
+      store_column<float, Ti::DB>(a.part + (part + first + c) * DP, acc, 1.0f, DP, lane);
+      if (h == 0) { a.ml[2 * (part + first + c)] = mt; a.ml[2 * (part + first + c) + 1] = l; }
     } else {
-      store_column<T, Ti::DB>(orow, acc, l == 0.0f ? 0.0f : 1.0f / l, a.D, lane);
-      if (h == 0 && a.lse) a.lse[at] = l == 0.0f ? __builtin_inff() : mt + log2f(l);
+      store_column<T, Ti::DB>(out_row(i, hh), acc, l == 0.0f ? 0.0f : 1.0f / l, a.D, lane);
+      if (h == 0 && a.lse) a.lse[first + c] = l == 0.0f ? __builtin_inff() : mt + log2f(l);
     }
   }
 }
 
-// joins the splits of the forward kernel: one thread per column and head element, splits in order
+// joins the splits of the forward kernel: a workgroup per column; its threads are DP head elements x shares of the parts
+constexpr int kAttnMaxSplits = 256;
 template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const AttnArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.B * a.G * a.C;
-  const int64_t at = t / DP;
-  const int d = (int)(t % DP);
-  if (at >= n) return;
-  float M = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.ml[2 * (s * n + at)]);
+  constexpr int Y = 256 / DP;
+  __shared__ float red[Y][DP], wt[kAttnMaxSplits], rm[4], rl[4];
+  const int64_t at = blockIdx.x, n = (int64_t)a.B * a.G * a.C;
+  const int t = threadIdx.x, d = t % DP, y = t / DP;
+  float mt = -__builtin_inff(), l = 0.0f;
+  if (t < a.splits) { mt = a.ml[2 * (t * n + at)]; l = a.ml[2 * (t * n + at) + 1]; }
+  float M = mt;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+  if ((t & 63) == 0) rm[t >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
   if (M == -__builtin_inff()) M = 0.0f;
-  float L = 0.0f, o = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = exp2f(a.ml[2 * (s * n + at)] - M);
-    L = fmaf(a.ml[2 * (s * n + at) + 1], f, L);
-    o = fmaf(a.part[(s * n + at) * DP + d], f, o);
-  }
+  const float f = exp2f(mt - M);
+  wt[t] = f;
+  l *= f;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
+  if ((t & 63) == 0) rl[t >> 6] = l;
+  __syncthreads();
+  const float L = (rl[0] + rl[1]) + (rl[2] + rl[3]);
+  float o = 0.0f;
+#pragma unroll 8
+  for (int s = y; s < a.splits; s += Y) o = fmaf(a.part[(s * n + at) * DP + d], wt[s], o);
+  red[y][d] = o;
+  __syncthreads();
+  if (y) return;
+  for (int x = 1; x < Y; ++x) o += red[x][d];
   const int bg = (int)(at / a.C), c = (int)(at % a.C), b = bg / a.G, gh = bg % a.G;
   int i, hh;
   col_of(a, c, i, hh);
@@ -525,36 +677,42 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_jo
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dq (and delta): columns = queries, keys and values stream
-template <typename T, int DP, bool WK> __global__ __launch_bounds__(256) void attn_dq_kernel(const AttnArgs a) {
-  using Sh = Shape<T, DP, WK>;
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))
+void attn_dq_kernel(const AttnArgs a) {
+  using Sh = Shape<T, DP, KW>;
   using Ti = Tile<T, DP>;
   constexpr int TR = Sh::TR, NS = Sh::NS;
   __shared__ __attribute__((aligned(16))) unsigned char lds[Sh::LDS];
   __shared__ __attribute__((aligned(16))) int hid[Sh::NBUF][TR];
-  __shared__ int red[8];
+  __shared__ int red[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-  const int ncb = (a.C + Sh::COLS - 1) / Sh::COLS;
-  unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int sp = (int)(id % (unsigned)a.splits);
-  id /= (unsigned)a.splits;
-  int cb = (int)(id % (unsigned)ncb);
-  const int bg = (int)(id / (unsigned)ncb), b = bg / a.G, gh = bg - b * a.G;
-  if (a.causal) cb = ncb - 1 - cb;
-  const int c0 = cb * Sh::COLS, c = c0 + (WK ? 0 : 32 * w) + (lane & 31);
+  const Place at = place_of(a, (a.C + Sh::COLS - 1) / Sh::COLS, true);
+  const int b = at.bg / a.G, gh = at.bg - b * a.G;
+  const int c0 = at.cb * Sh::COLS, c = c0 + (KW == 1 ? 32 * w : 0) + (lane & 31);
   const bool mine = c < a.C;
+  const uint8_t *pad = a.pad ? a.pad + (int64_t)b * a.pad_b : nullptr;
+  int lo, hi, first_limit;
+  key_range(a, at.sp, TR, c0, Sh::COLS, lo, hi, first_limit);
+  auto tile = [&](int buf, int which) { return reinterpret_cast<T *>(lds + (2 * buf + which) * Sh::TILE); };
+  clear_tiles<2 * Sh::NBUF * Sh::TILE>(lds, a.DL < DP);
+  KeyRows<T, DP, TR> st;
+  st.kb = static_cast<const T *>(a.k) + (int64_t)b * a.ks[0] + (int64_t)gh * a.ks[2];
+  st.vb = static_cast<const T *>(a.v) + (int64_t)b * a.vs[0] + (int64_t)gh * a.vs[2];
+  auto issue = [&](int t0, int buf) { st.issue(a, pad, lo, t0, hi, tile(buf, 0), tile(buf, 1)); };
+  if (lo < hi) issue(lo, 0);
+
+  const Lanes<T, DP> ln(lane);
+  typename Ti::Columns q, g;
   int i, hh;
   col_of(a, mine ? c : 0, i, hh);
   const int head = gh * a.HG + hh;
-  const T *kb = static_cast<const T *>(a.k) + (int64_t)b * a.ks[0] + (int64_t)gh * a.ks[2];
-  const T *vb = static_cast<const T *>(a.v) + (int64_t)b * a.vs[0] + (int64_t)gh * a.vs[2];
-  const uint8_t *pad = a.pad ? a.pad + (int64_t)b * a.pad_b : nullptr;
-  uint4 q[Ti::KK], g[Ti::KK];
   load_columns<T, DP>(q, mine ? static_cast<const T *>(a.q) + (int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)head * a.qs[2]
-                              : nullptr, a.D, a.qvec, lane);
+                              : nullptr, a.DL, lane);
   load_columns<T, DP>(g, mine ? static_cast<const T *>(a.g) + (int64_t)b * a.gs[0] + (int64_t)i * a.gs[1] + (int64_t)head * a.gs[2]
-                              : nullptr, a.D, a.gvec, lane);
-  const int64_t at = (int64_t)bg * a.C + c;
-  const int64_t row_at = (((int64_t)b * a.L + i) * a.H + head) * a.D;
+                              : nullptr, a.DL, lane);
+  const int64_t row_at = (((int64_t)b * a.L + i) * a.H + head) * a.D, col_at = (int64_t)at.bg * a.C + c;
+  const int lim = a.causal ? i + a.S - a.L : a.S;
   float delta = 0.0f;
   if (mine) {
     const T *orow = static_cast<const T *>(a.o) + row_at;
@@ -563,185 +721,130 @@ template <typename T, int DP, bool WK> __global__ __launch_bounds__(256) void at
       delta += dot_piece<T>(g[kk], load_piece<T>(orow, kk * Elem<T>::KS + h * (Elem<T>::KS / 2), a.D, a.ovec));
   }
   delta += other_half(delta);
-  if (mine && h == 0 && sp == 0 && (!WK || w == 0)) a.delta[at] = delta;
-  const float lse = mine ? a.lse[at] : __builtin_inff();
-
-  int lo = 0, hi = a.S, first_limit = a.S;
-  if (a.splits > 1) {
-    const int chunk = ((a.S + a.splits - 1) / a.splits + TR - 1) / TR * TR;
-    lo = (int)min((int64_t)sp * chunk, (int64_t)a.S);
-    hi = min(lo + chunk, a.S);
-  }
-  const int lim = a.causal ? i + a.S - a.L : a.S;
-  if (a.causal) {
-    int il, ih;
-    col_of(a, min(c0 + Sh::COLS, a.C) - 1, il, ih);
-    hi = min(hi, il + a.S - a.L + 1);
-    col_of(a, c0, il, ih);
-    first_limit = il + a.S - a.L;
-  }
-  if (pad && lo < hi) visible_range(pad, lo, hi, red);
+  const float lse = mine ? a.lse[col_at] : __builtin_inff();
+  if (mine && h == 0 && at.sp == 0 && (KW == 1 || w == 0)) a.delta[col_at] = delta;
+  if (pad && lo < hi) hi = visible_end(pad, lo, hi, red);
 
   f32x16 acc[Ti::DB];
 #pragma unroll
   for (int db = 0; db < Ti::DB; ++db) acc[db] = f32x16{0.0f};
   ColumnScale<T, Ti::DB> cs;
   cs.start();
-  Stage<T, DP, TR> sk, sv;
-  int hidden = 0;
-  auto fetch = [&](int t0) {
-    sk.fetch([&](int j) -> const T * { return j < hi && !(pad && pad[j]) ? kb + (int64_t)j * a.ks[1] : nullptr; }, t0, a.D, a.kvec);
-    sv.fetch([&](int j) -> const T * { return j < hi && !(pad && pad[j]) ? vb + (int64_t)j * a.vs[1] : nullptr; }, t0, a.D, a.vvec);
-    if ((int)threadIdx.x < TR) hidden = t0 + (int)threadIdx.x >= hi || (pad && pad[t0 + (int)threadIdx.x]);
-  };
-  auto put = [&](int buf) {
-    sk.store(reinterpret_cast<T *>(lds + (2 * buf) * Sh::TILE));
-    sv.store(reinterpret_cast<T *>(lds + (2 * buf + 1) * Sh::TILE));
-    if ((int)threadIdx.x < TR) hid[buf][threadIdx.x] = hidden;
-  };
   auto compute = [&](int t0, int buf) {
-    const T *tk = reinterpret_cast<const T *>(lds + (2 * buf) * Sh::TILE);
-    const T *tv = reinterpret_cast<const T *>(lds + (2 * buf + 1) * Sh::TILE);
-    const int r0 = WK ? 32 * NS * w : 0;
+    const T *tk = tile(buf, 0), *tv = tile(buf, 1);
     const bool some_hidden = pad || t0 + TR > hi || t0 + TR - 1 > first_limit;
-    float ds[NS][16];
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < NS; ++n) {
+      const int r0 = 32 * ((KW == 1 ? 0 : NS * w) + n);
       f32x16 x = f32x16{0.0f}, y = f32x16{0.0f};
 #pragma unroll
       for (int kk = 0; kk < Ti::KK; ++kk) {
-        mma(x, frag_rows<T, DP>(tk, r0 + 32 * n, kk, lane), q[kk], T());
-        mma(y, frag_rows<T, DP>(tv, r0 + 32 * n, kk, lane), g[kk], T());
+        mma(x, ln.rows(tk, r0, kk), q[kk], T());
+        mma(y, ln.rows(tv, r0, kk), g[kk], T());
       }
+      read_ahead<2 * Ti::KK, 2 * Ti::KK * Elem<T>::MMA, Sh::AHEAD>();
+      uint4 fk[Ti::DB];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[n][r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c2, -lse)) * (y[r] - delta);
+      for (int db = 0; db < Ti::DB; ++db) fk[db] = ln.cols(tk, r0, db, 0);
+      float ds[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c2, -lse)) * (y[r] - delta);
       if (some_hidden) {
+        rare();
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int row = r0 + 32 * n + 8 * r4 + 4 * h;
-          const int4 hd = *reinterpret_cast<const int4 *>(&hid[buf][row]);
-          const int hx[4] = {hd.x, hd.y, hd.z, hd.w};
+          const int row = r0 + 8 * r4 + 4 * h;
+          const int4 hv = *reinterpret_cast<const int4 *>(&hid[buf][row]);
+          const int hx[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (hx[e] || t0 + row + e > lim) ds[n][4 * r4 + e] = 0.0f;
+            if (hx[e] || t0 + row + e > lim) ds[4 * r4 + e] = 0.0f;
+        }
+      }
+      cs.apply(ds, acc);
+#pragma unroll
+      for (int kk = 0; kk < Ti::RK; ++kk) {
+        const uint4 p = row_frag<T>(ds, kk);
+#pragma unroll
+        for (int db = 0; db < Ti::DB; ++db) {
+          mma(acc[db], fk[db], p, T());
+          if (kk + 1 < Ti::RK) fk[db] = ln.cols(tk, r0, db, kk + 1);
         }
       }
     }
-    cs.apply(ds, acc);
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int kk = 0; kk < Ti::RK; ++kk) {
-        const uint4 p = row_frag<T>(ds[n], kk);
-#pragma unroll
-        for (int db = 0; db < Ti::DB; ++db) mma(acc[db], frag_cols<T, DP>(tk, r0 + 32 * n, db, kk, lane), p, T());
-      }
   };
-  if (lo < hi) {
-    fetch(lo);
-    if (Sh::NBUF == 2) put(0);
-    int buf = 0;
-    for (int t0 = lo; t0 < hi; t0 += TR) {
-      const bool more = t0 + TR < hi;
-      if (Sh::NBUF == 2) {
-        if (more) fetch(t0 + TR);
-        __syncthreads();
-        compute(t0, buf);
-        if (more) put(buf ^ 1);
-        buf ^= 1;
-      } else {
-        __syncthreads();
-        put(0);
-        __syncthreads();
-        if (more) fetch(t0 + TR);
-        compute(t0, 0);
-      }
-    }
-  }
+  stream<TR, Sh::NBUF>(lo, hi, issue, [&](int buf) { st.land(tile(buf, 0), tile(buf, 1), hid[buf]); }, compute);
+
   const float f = a.scale / cs.f;
-  if constexpr (WK) {
+  const int64_t part = (int64_t)at.sp * a.B * a.G * a.C;
+  if constexpr (KW > 1) {
+    float *jo = reinterpret_cast<float *>(lds);
     __syncthreads();
-    join_put<DP>(reinterpret_cast<float *>(lds), acc, f, w, lane);
+    join_put<DP>(jo, acc, f, w, lane);
     __syncthreads();
     for (int t = threadIdx.x; t < 32 * DP; t += 256) {
       const int col = t / DP, d = t % DP, cc = c0 + col;
       if (cc >= a.C || d >= a.D) continue;
-      const float o = join_get<DP>(reinterpret_cast<const float *>(lds), col, d);
+      const float o = join_get<DP>(jo, col, d);
       int ci, ch;
       col_of(a, cc, ci, ch);
-      if (a.splits > 1)
-        a.part[((int64_t)sp * a.B * a.G * a.C + (int64_t)bg * a.C + cc) * DP + d] = o;
-      else
-        static_cast<T *>(a.out)[(((int64_t)b * a.L + ci) * a.H + gh * a.HG + ch) * a.D + d] = (T)o;
+      if (a.splits > 1) a.part[(part + (int64_t)at.bg * a.C + cc) * DP + d] = o;
+      else static_cast<T *>(a.out)[(((int64_t)b * a.L + ci) * a.H + gh * a.HG + ch) * a.D + d] = (T)o;
     }
   } else if (mine) {
-    if (a.splits > 1)
-      store_column<float, Ti::DB>(a.part + ((int64_t)sp * a.B * a.G * a.C + at) * DP, acc, f, DP, lane);
-    else
-      store_column<T, Ti::DB>(static_cast<T *>(a.out) + row_at, acc, f, a.D, lane);
+    if (a.splits > 1) store_column<float, Ti::DB>(a.part + (part + col_at) * DP, acc, f, DP, lane);
+    else store_column<T, Ti::DB>(static_cast<T *>(a.out) + row_at, acc, f, a.D, lane);
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dk and dv: columns = keys, the queries that use this key head and their output gradients stream; the heads of a
 // group are rows of the same stream, so shared heads are summed here, in a fixed order and without atomics
-template <typename T, int DP, bool WK> __global__ __launch_bounds__(256) void attn_dkv_kernel(const AttnArgs a) {
-  using Sh = Shape<T, DP, WK>;
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WB)))
+void attn_dkv_kernel(const AttnArgs a) {
+  using Sh = Shape<T, DP, KW>;
   using Ti = Tile<T, DP>;
   constexpr int TR = Sh::TR, NS = Sh::NS;
   __shared__ __attribute__((aligned(16))) unsigned char lds[Sh::LDS];
   __shared__ __attribute__((aligned(16))) float slse[Sh::NBUF][TR], sdel[Sh::NBUF][TR];
   __shared__ __attribute__((aligned(16))) int slim[Sh::NBUF][TR];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-  const int nkb = (a.S + Sh::COLS - 1) / Sh::COLS;
-  unsigned id = xcd_order(blockIdx.x, gridDim.x);
-  const int sp = (int)(id % (unsigned)a.splits);
-  id /= (unsigned)a.splits;
-  const int kblk = (int)(id % (unsigned)nkb), bg = (int)(id / (unsigned)nkb), b = bg / a.G, gh = bg - b * a.G;
-  const int j0 = kblk * Sh::COLS, j = j0 + (WK ? 0 : 32 * w) + (lane & 31);
+  const Place at = place_of(a, (a.S + Sh::COLS - 1) / Sh::COLS, false);          // (the first keys are seen by the most queries)
+  const int b = at.bg / a.G, gh = at.bg - b * a.G;
+  const int j0 = at.cb * Sh::COLS, j = j0 + (KW == 1 ? 32 * w : 0) + (lane & 31);
   const bool mine = j < a.S, seen = mine && !(a.pad && a.pad[(int64_t)b * a.pad_b + j]);
-  const T *qb = static_cast<const T *>(a.q) + (int64_t)b * a.qs[0] + (int64_t)gh * a.HG * a.qs[2];
-  const T *gb = static_cast<const T *>(a.g) + (int64_t)b * a.gs[0] + (int64_t)gh * a.HG * a.gs[2];
-  const float *lb = a.lse + (int64_t)bg * a.C, *db_ = a.delta + (int64_t)bg * a.C;
-  uint4 k[Ti::KK], v[Ti::KK];
-  load_columns<T, DP>(k, seen ? static_cast<const T *>(a.k) + (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)gh * a.ks[2]
-                              : nullptr, a.D, a.kvec, lane);
-  load_columns<T, DP>(v, seen ? static_cast<const T *>(a.v) + (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)gh * a.vs[2]
-                              : nullptr, a.D, a.vvec, lane);
-  // columns (queries) of this workgroup; a workgroup whose keys are all padding has none
+  // columns (queries) of this workgroup
   int lo = 0, hi = a.C;
   if (a.splits > 1) {
     const int chunk = ((a.C + a.splits - 1) / a.splits + TR - 1) / TR * TR;
-    lo = (int)min((int64_t)sp * chunk, (int64_t)a.C);
-    hi = min(lo + chunk, a.C);
+    hi = (int)max(a.C - (int64_t)at.sp * chunk, (int64_t)0);
+    lo = max(hi - chunk, 0);
   }
   if (a.causal) {                                                     // the first query that sees key j0
     const int64_t i0 = (int64_t)j0 - (a.S - a.L);
-    if (i0 > 0) lo = (int)max((int64_t)lo, min(i0 * a.HG, (int64_t)a.C) / TR * TR);
+    if (i0 > 0) lo = (int)max((int64_t)lo, min(i0 * a.HG, (int64_t)a.C));
   }
-  if (!__syncthreads_or(seen)) hi = lo;
-
-  f32x16 ak[Ti::DB], av[Ti::DB];
-#pragma unroll
-  for (int db = 0; db < Ti::DB; ++db) { ak[db] = f32x16{0.0f}; av[db] = f32x16{0.0f}; }
-  ColumnScale<T, Ti::DB> cs;
-  cs.start();
-  Stage<T, DP, TR> sq, sg;
+  auto tile = [&](int buf, int which) { return reinterpret_cast<T *>(lds + (2 * buf + which) * Sh::TILE); };
+  clear_tiles<2 * Sh::NBUF * Sh::TILE>(lds, a.DL < DP);
+  Rows<T, DP, TR> sq, sg;
   float rl = 0.0f, rd = 0.0f;
   int rlim = 0;
-  auto fetch = [&](int t0) {
-    sq.fetch([&](int c) -> const T * {
-      if (c >= hi) return nullptr;
-      int i, hh;
-      col_of(a, c, i, hh);
-      return qb + (int64_t)i * a.qs[1] + (int64_t)hh * a.qs[2];
-    }, t0, a.D, a.qvec);
-    sg.fetch([&](int c) -> const T * {
-      if (c >= hi) return nullptr;
-      int i, hh;
-      col_of(a, c, i, hh);
-      return gb + (int64_t)i * a.gs[1] + (int64_t)hh * a.gs[2];
-    }, t0, a.D, a.gvec);
+  const bool even = TR % a.HG == 0;                                   // a tile is a whole number of query positions
+  const T *qb = static_cast<const T *>(a.q) + (int64_t)b * a.qs[0] + (int64_t)gh * a.HG * a.qs[2];
+  const T *gb = static_cast<const T *>(a.g) + (int64_t)b * a.gs[0] + (int64_t)gh * a.HG * a.gs[2];
+  const float *lb = a.lse + (int64_t)at.bg * a.C, *db_ = a.delta + (int64_t)at.bg * a.C;
+  auto issue = [&](int t0, int buf) {
+    if (t0 == lo || t0 + TR > hi || !even) {
+      sq.place([&](int c) { int i, hh; col_of(a, c, i, hh); return qb + (int64_t)i * a.qs[1] + (int64_t)hh * a.qs[2]; }, t0, hi);
+      sg.place([&](int c) { int i, hh; col_of(a, c, i, hh); return gb + (int64_t)i * a.gs[1] + (int64_t)hh * a.gs[2]; }, t0, hi);
+    } else {
+      const int64_t by = TR / a.HG;
+      sq.advance(by * a.qs[1]);
+      sg.advance(by * a.gs[1]);
+    }
+    sq.issue(tile(buf, 0), a.DL);
+    sg.issue(tile(buf, 1), a.DL);
     if ((int)threadIdx.x < TR) {
       const int c = t0 + (int)threadIdx.x;
       rl = c < hi ? lb[c] : __builtin_inff();
@@ -751,113 +854,113 @@ template <typename T, int DP, bool WK> __global__ __launch_bounds__(256) void at
       rlim = a.causal ? i + a.S - a.L : a.S;
     }
   };
-  auto put = [&](int buf) {
-    sq.store(reinterpret_cast<T *>(lds + (2 * buf) * Sh::TILE));
-    sg.store(reinterpret_cast<T *>(lds + (2 * buf + 1) * Sh::TILE));
-    if ((int)threadIdx.x < TR) { slse[buf][threadIdx.x] = rl; sdel[buf][threadIdx.x] = rd; slim[buf][threadIdx.x] = rlim; }
-  };
-  auto compute = [&](int t0, int buf) {
-    const T *tq = reinterpret_cast<const T *>(lds + (2 * buf) * Sh::TILE);
-    const T *tg = reinterpret_cast<const T *>(lds + (2 * buf + 1) * Sh::TILE);
-    const int r0 = WK ? 32 * NS * w : 0;
-    int il = 0, ih;
-    if (a.causal) col_of(a, t0, il, ih);
-    const bool some_hidden = a.causal && j0 + Sh::COLS - 1 > il + a.S - a.L;
+  if (lo < hi) issue(lo, 0);
+  const Lanes<T, DP> ln(lane);
+  typename Ti::Columns k, v;
+  load_columns<T, DP>(k, seen ? static_cast<const T *>(a.k) + (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)gh * a.ks[2]
+                              : nullptr, a.DL, lane);
+  load_columns<T, DP>(v, seen ? static_cast<const T *>(a.v) + (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)gh * a.vs[2]
+                              : nullptr, a.DL, lane);
+  if (a.pad && !__builtin_amdgcn_readfirstlane(__syncthreads_or(seen))) hi = lo;   // all of its keys are padding
+
+  f32x16 ak[Ti::DB], av[Ti::DB];
 #pragma unroll
+  for (int db = 0; db < Ti::DB; ++db) { ak[db] = f32x16{0.0f}; av[db] = f32x16{0.0f}; }
+  ColumnScale<T, Ti::DB> cs;
+  cs.start();
+  auto compute = [&](int t0, int buf) {
+    const T *tq = tile(buf, 0), *tg = tile(buf, 1);
+    int il = 0, ih;
+    if (a.causal) col_of(a, t0, il, ih);                              // (the tile's first query)
+    const bool some_hidden = a.causal && j0 + Sh::COLS - 1 > il + a.S - a.L;
+#pragma unroll 1
     for (int n = 0; n < NS; ++n) {
+      const int r0 = 32 * ((KW == 1 ? 0 : NS * w) + n);
       f32x16 x = f32x16{0.0f}, y = f32x16{0.0f};
 #pragma unroll
       for (int kk = 0; kk < Ti::KK; ++kk) {
-        mma(x, frag_rows<T, DP>(tq, r0 + 32 * n, kk, lane), k[kk], T());
-        mma(y, frag_rows<T, DP>(tg, r0 + 32 * n, kk, lane), v[kk], T());
+        mma(x, ln.rows(tq, r0, kk), k[kk], T());
+        mma(y, ln.rows(tg, r0, kk), v[kk], T());
       }
-      float p[16], ds[1][16];
+      read_ahead<2 * Ti::KK, 2 * Ti::KK * Elem<T>::MMA, Sh::AHEAD>();
+      uint4 fg[Ti::DB], fq[Ti::DB];
+#pragma unroll
+      for (int db = 0; db < Ti::DB; ++db) { fg[db] = ln.cols(tg, r0, db, 0); fq[db] = ln.cols(tq, r0, db, 0); }
+      float p[16], ds[16];
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const int row = r0 + 32 * n + 8 * r4 + 4 * h;
+        const int row = r0 + 8 * r4 + 4 * h;
         const float4 ls = *reinterpret_cast<const float4 *>(&slse[buf][row]);
         const float4 de = *reinterpret_cast<const float4 *>(&sdel[buf][row]);
         const float lx[4] = {ls.x, ls.y, ls.z, ls.w}, dx[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = 4 * r4 + e;
-          p[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c2, -lx[e]));
-          ds[0][r] = y[r] - dx[e];
+          p[4 * r4 + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * r4 + e], a.c2, -lx[e]));
+          ds[4 * r4 + e] = y[4 * r4 + e] - dx[e];
         }
-        if (some_hidden) {
-          const int4 lm = *reinterpret_cast<const int4 *>(&slim[buf][row]);
+      }
+      if (some_hidden) {
+        rare();
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int4 lm = *reinterpret_cast<const int4 *>(&slim[buf][r0 + 8 * r4 + 4 * h]);
           const int mx[4] = {lm.x, lm.y, lm.z, lm.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (j > mx[e]) { p[4 * r4 + e] = 0.0f; ds[0][4 * r4 + e] = 0.0f; }
+            if (j > mx[e]) { p[4 * r4 + e] = 0.0f; ds[4 * r4 + e] = 0.0f; }
         }
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[0][r] *= p[r];
-      if constexpr (prob_shift<T>() != 0.0f) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] *= 32768.0f;
+      for (int r = 0; r < 16; ++r) {
+        ds[r] *= p[r];
+        if (prob_shift<T>() != 0.0f) p[r] *= 32768.0f;                // (the probability in a float16 product carries 2^15)
       }
       cs.apply(ds, ak);
 #pragma unroll
       for (int kk = 0; kk < Ti::RK; ++kk) {
-        const uint4 pf = row_frag<T>(p, kk), df = row_frag<T>(ds[0], kk);
+        const uint4 pf = row_frag<T>(p, kk), df = row_frag<T>(ds, kk);
 #pragma unroll
         for (int db = 0; db < Ti::DB; ++db) {
-          mma(av[db], frag_cols<T, DP>(tg, r0 + 32 * n, db, kk, lane), pf, T());
-          mma(ak[db], frag_cols<T, DP>(tq, r0 + 32 * n, db, kk, lane), df, T());
+          mma(av[db], fg[db], pf, T());
+          mma(ak[db], fq[db], df, T());
+          if (kk + 1 < Ti::RK) { fg[db] = ln.cols(tg, r0, db, kk + 1); fq[db] = ln.cols(tq, r0, db, kk + 1); }
         }
       }
     }
   };
-  if (lo < hi) {
-    fetch(lo);
-    if (Sh::NBUF == 2) put(0);
-    int buf = 0;
-    for (int t0 = lo; t0 < hi; t0 += TR) {
-      const bool more = t0 + TR < hi;
-      if (Sh::NBUF == 2) {
-        if (more) fetch(t0 + TR);
-        __syncthreads();
-        compute(t0, buf);
-        if (more) put(buf ^ 1);
-        buf ^= 1;
-      } else {
-        __syncthreads();
-        put(0);
-        __syncthreads();
-        if (more) fetch(t0 + TR);
-        compute(t0, 0);
-      }
-    }
-  }
+  stream<TR, Sh::NBUF>(
+      lo, hi, issue,
+      [&](int buf) {
+        if ((int)threadIdx.x < TR) { slse[buf][threadIdx.x] = rl; sdel[buf][threadIdx.x] = rd; slim[buf][threadIdx.x] = rlim; }
+      },
+      compute);
+
   // (a padded key's lane has computed with zeros for its key and value: its sums are dropped)
-  const float fk = seen ? a.scale / cs.f : 0.0f, fv = seen ? exp2f(-prob_shift<T>()) : 0.0f;
+  const float fk = a.scale / cs.f, fv = exp2f(-prob_shift<T>());
   if (!seen) {
 #pragma unroll
     for (int db = 0; db < Ti::DB; ++db) { ak[db] = f32x16{0.0f}; av[db] = f32x16{0.0f}; }
   }
-  if constexpr (WK) {
+  const int64_t part = ((int64_t)at.sp * a.B * a.G + at.bg) * a.S;
+  if constexpr (KW > 1) {
+    float *jo = reinterpret_cast<float *>(lds);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
-      join_put<DP>(reinterpret_cast<float *>(lds), which ? av : ak, which ? fv : fk, w, lane);
+      join_put<DP>(jo, which ? av : ak, which ? fv : fk, w, lane);
       __syncthreads();
       for (int t = threadIdx.x; t < 32 * DP; t += 256) {
         const int col = t / DP, d = t % DP, jj = j0 + col;
         if (jj >= a.S || d >= a.D) continue;
-        const float o = join_get<DP>(reinterpret_cast<const float *>(lds), col, d);
-        if (a.splits > 1)
-          (which ? a.part2 : a.part)[(((int64_t)sp * a.B * a.G + bg) * a.S + jj) * DP + d] = o;
-        else
-          static_cast<T *>(which ? a.out2 : a.out)[(((int64_t)b * a.S + jj) * a.G + gh) * a.D + d] = (T)o;
+        const float o = join_get<DP>(jo, col, d);
+        if (a.splits > 1) (which ? a.part2 : a.part)[(part + jj) * DP + d] = o;
+        else static_cast<T *>(which ? a.out2 : a.out)[(((int64_t)b * a.S + jj) * a.G + gh) * a.D + d] = (T)o;
       }
     }
   } else if (mine) {
     if (a.splits > 1) {
-      const int64_t row = (((int64_t)sp * a.B * a.G + bg) * a.S + j) * DP;
-      store_column<float, Ti::DB>(a.part + row, ak, fk, DP, lane);
-      store_column<float, Ti::DB>(a.part2 + row, av, fv, DP, lane);
+      store_column<float, Ti::DB>(a.part + (part + j) * DP, ak, fk, DP, lane);
+      store_column<float, Ti::DB>(a.part2 + (part + j) * DP, av, fv, DP, lane);
     } else {
       const int64_t row = (((int64_t)b * a.S + j) * a.G + gh) * a.D;
       store_column<T, Ti::DB>(static_cast<T *>(a.out) + row, ak, fk, a.D, lane);
@@ -881,50 +984,67 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float *part, int sp
   out[((((int64_t)b * (n / per) + c / per) * G + gh) * per + c % per) * D + d] = (T)s;
 }
 
+// rows whose 16-byte pieces are not aligned, copied into aligned ones of DL elements (zeros past D): [B, n, heads, DL]
+template <typename T>
+__global__ __launch_bounds__(256) void attn_pack_kernel(const T *from, int64_t sb, int64_t sl, int64_t sh, int64_t rows, int n,
+                                                        int heads, int D, int DL, T *to) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * DL; t += (int64_t)gridDim.x * 256) {
+    const int64_t row = t / DL;
+    const int d = (int)(t - row * DL), hd = (int)(row % heads);
+    const int64_t i = row / heads, b = i / n;
+    to[t] = d < D ? from[b * sb + (i - b * n) * sl + hd * sh + d] : (T)0.0f;
+  }
+}
+
 // ---- launches ---------------------------------------------------------------------------------------------------------
 enum AttnPass { kAttnFwd, kAttnDq, kAttnDkv };
 
-template <typename T, int DP, bool WK> void attn_launch(AttnPass pass, const AttnArgs &a, hipStream_t s) {
-  const int cols = pass == kAttnDkv ? a.S : a.C, per = Shape<T, DP, WK>::COLS;
+template <typename T, int DP, int KW, bool DKV> void attn_launch(AttnPass pass, const AttnArgs &a, hipStream_t s) {
+  const int cols = DKV ? a.S : a.C, per = Shape<T, DP, KW>::COLS;
   const unsigned grid = (unsigned)((int64_t)a.B * a.G * ((cols + per - 1) / per) * a.splits);
-  if (pass == kAttnFwd)
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, WK>), dim3(grid), dim3(256), 0, s, a);
-  else if (pass == kAttnDq)
-    hipLaunchKernelGGL((attn_dq_kernel<T, DP, WK>), dim3(grid), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, WK>), dim3(grid), dim3(256), 0, s, a);
+  if constexpr (DKV) {
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, KW>), dim3(grid), dim3(256), 0, s, a);
+  } else if (pass == kAttnFwd) {
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, KW>), dim3(grid), dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP, KW>), dim3(grid), dim3(256), 0, s, a);
+  }
 }
 
-template <typename T, int DP> int attn_run(AttnPass pass, const AttnArgs &a, bool wk, hipStream_t s) {
-  if (wk) attn_launch<T, DP, true>(pass, a, s);
-  else attn_launch<T, DP, false>(pass, a, s);
+template <typename T, int DP, bool DKV> int attn_run(AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s) {
+  if (shared) attn_launch<T, DP, 4, DKV>(pass, a, s);
+  else attn_launch<T, DP, 1, DKV>(pass, a, s);
   HSGK_LAUNCH_CHECK();
   if (a.splits > 1) {
-    const int n = pass == kAttnDkv ? a.S : a.C;
-    const unsigned grid = (unsigned)(((int64_t)a.B * a.G * n * DP + 255) / 256);
-    if (pass == kAttnFwd) {
-      hipLaunchKernelGGL((attn_fwd_join_kernel<T, DP>), dim3(grid), dim3(256), 0, s, a);
-    } else {
-      const int per = pass == kAttnDkv ? 1 : a.HG;
+    const int n = DKV ? a.S : a.C, per = DKV ? 1 : a.HG;
+    const int64_t rows = (int64_t)a.B * a.G * n;
+    const unsigned grid = (unsigned)((rows * DP + 255) / 256);
+    if (pass == kAttnFwd)
+      hipLaunchKernelGGL((attn_fwd_join_kernel<T, DP>), dim3((unsigned)rows), dim3(256), 0, s, a);
+    else
       hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3(grid), dim3(256), 0, s, a.part, a.splits, a.B, a.G, n, per, a.D,
                          static_cast<T *>(a.out));
-      if (pass == kAttnDkv)
-        hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3(grid), dim3(256), 0, s, a.part2, a.splits, a.B, a.G, n, per, a.D,
-                           static_cast<T *>(a.out2));
-    }
+    if (DKV)
+      hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3(grid), dim3(256), 0, s, a.part2, a.splits, a.B, a.G, n, per, a.D,
+                         static_cast<T *>(a.out2));
     HSGK_LAUNCH_CHECK();
   }
   return 0;
 }
 
-template <typename T> int attn_type(AttnPass pass, const AttnArgs &a, bool wk, hipStream_t s) {
-  if (a.D <= 32) return attn_run<T, 32>(pass, a, wk, s);
-  if (a.D <= 64) return attn_run<T, 64>(pass, a, wk, s);
-  return attn_run<T, 128>(pass, a, wk, s);
+template <typename T, bool DKV> int attn_type(AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s) {
+  if (a.D <= 32) return attn_run<T, 32, DKV>(pass, a, shared, s);
+  if (a.D <= 64) return attn_run<T, 64, DKV>(pass, a, shared, s);
+  return attn_run<T, 128, DKV>(pass, a, shared, s);
 }
 
-int attn_f32(AttnPass pass, const AttnArgs &a, bool wk, hipStream_t s);
-int attn_bf16(AttnPass pass, const AttnArgs &a, bool wk, hipStream_t s);
-int attn_f16(AttnPass pass, const AttnArgs &a, bool wk, hipStream_t s);
+// one translation unit a type and side, so that they build next to each other
+#define HSGK_ATTN(name) int name(AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s)
+HSGK_ATTN(attn_f32);
+HSGK_ATTN(attn_bf16);
+HSGK_ATTN(attn_f16);
+HSGK_ATTN(attn_dkv_f32);
+HSGK_ATTN(attn_dkv_bf16);
+HSGK_ATTN(attn_dkv_f16);
 
 }  // namespace hsgk

@@ -66,89 +66,153 @@ template <typename T> struct Piece {
   static constexpr int E = 16 / (int)sizeof(T);
 };
 
-// the E elements from e0 on of a row of V, 16 bytes at once where they are all inside (e0 is chosen so that the address
-// is aligned); `fill` elsewhere
-template <typename T>
-__device__ __forceinline__ void get_piece(const T *row, int64_t e0, int64_t V, float fill, float (&x)[Piece<T>::E]) {
-  constexpr int E = Piece<T>::E;
-  if (e0 >= 0 && e0 + E <= V) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(row + e0);
-    T y[E];
-    __builtin_memcpy(y, &u, 16);
-#pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = (float)y[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = e0 + i >= 0 && e0 + i < V ? (float)row[e0 + i] : fill;
+// a row cut into 16-byte pieces at aligned addresses: `head` elements before the first, `full` pieces, the rest from
+// element `rest` on.  Piece 0 lies `skip` pieces behind a 128-byte line's start; the threads are counted from there, so that
+// what a wave moves at once begins and ends with a line.
+template <typename T> struct Cut {
+  int head, full, rest, skip;
+  __device__ __forceinline__ Cut(const T *row, int V) {
+    constexpr int E = Piece<T>::E;
+    head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    if (head > V) head = V;
+    full = (V - head) / E;
+    rest = head + full * E;
+    skip = (int)(reinterpret_cast<uintptr_t>(row + head) >> 4) & 7;
   }
+};
+
+typedef unsigned u32x4nt __attribute__((ext_vector_type(4)));
+
+// Whether a row is read past the caches: forward and backward both read the logits, so the forward leaves them in the
+// 256 MB cache where they fit; larger ones would only push each other out.  (forward + backward, us: 308 MB past 45 + 106,
+// through 68 + 116; 206 MB past 43 + 100, through 43 + 73.)
+template <bool NT> __device__ __forceinline__ uint4 load16(const uint4 *p) {
+  return NT ? __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4nt *>(p))) : *p;
 }
 
-// teacher: probabilities of the row's entries into tp, their indices into ti (-1: does not count); returns whether any counts
-template <int P>
-__device__ __forceinline__ bool teacher_row(const DistillArgs &a, int64_t row, int t, float *tp, int64_t *ti, float *red,
-                                            float &top, float &mass) {
-  float m = -__builtin_inff();
-  for (int j = t; j < a.k; j += P) {
-    const float x = a.t[row * a.k + j];
-    const int64_t v = a.idx[row * a.k + j];
-    const bool ok = v >= 0 && v < a.V && !(x == -__builtin_inff());
-    ti[j] = ok ? v : -1;
-    tp[j] = x;
-    if (ok) m = fmaxf(m, x != x ? __builtin_inff() : x);
-  }
-  m = row_max<P>(m, red);
-  top = m;
-  const bool some = m > -__builtin_inff();
-  float s = 0.0f;
-  for (int j = t; j < a.k; j += P) {
-    const float p = ti[j] >= 0 ? __builtin_amdgcn_exp2f((tp[j] - m) * a.c2) : 0.0f;
-    s += p;
-  }
-  mass = row_sum<P>(s, red);
-  return some;
+// exp2 of (x - base) / T.  Logits of 16 bits take one instruction for the argument (base2 = base c2 rounded: 2^-24 of an
+// exponent's size, the same for the whole row); float32 subtracts first.
+template <typename T> __device__ __forceinline__ float power(float x, float base, float base2, float c2) {
+  return __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(x, c2, -base2) : (x - base) * c2);
 }
 
-template <typename T, int P> __global__ __launch_bounds__(256) void distill_fwd_kernel(const DistillArgs a) {
+template <typename T> __device__ __forceinline__ void widen(const uint4 &u, float (&x)[Piece<T>::E]) {
+  T y[Piece<T>::E];
+  __builtin_memcpy(y, &u, 16);
+#pragma unroll
+  for (int i = 0; i < Piece<T>::E; ++i) x[i] = (float)y[i];
+}
+
+// the teacher's entries of a row, P apart in the threads of the row: value, index (-1: does not count), the student's
+// logit there.  load() only sends for them; the row itself is on its way before gather() looks at an index.
+template <int P> struct Teacher {
+  static constexpr int N = kDistillMax / P;
+  float t[N], z[N];
+  int64_t at[N];
+  int v[N];
+  float top, mass;
+  __device__ __forceinline__ void load(const DistillArgs &a, int64_t row, int th) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int j = th + n * P;
+      at[n] = -1;
+      t[n] = -__builtin_inff();
+      if (j < a.k) {
+        at[n] = a.idx[row * a.k + j];
+        t[n] = a.t[row * a.k + j];
+      }
+    }
+  }
+  template <typename T> __device__ __forceinline__ void gather(const DistillArgs &a, const T *zrow) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = at[n] >= 0 && at[n] < a.V && !(t[n] == -__builtin_inff()) ? (int)at[n] : -1;
+      z[n] = v[n] >= 0 ? (float)zrow[v[n]] : 0.0f;
+    }
+  }
+  // maximum and mass; whether any entry counts.  A NaN among them reaches the mass.
+  __device__ __forceinline__ bool sum(const DistillArgs &a, float *red) {
+    float m = -__builtin_inff(), s = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (v[n] >= 0) m = fmaxf(m, t[n] != t[n] ? __builtin_inff() : t[n]);
+    top = row_max<P>(m, red);
+#pragma unroll
+    for (int n = 0; n < N; ++n) s += weight(a, n);
+    mass = row_sum<P>(s, red);
+    return top > -__builtin_inff();
+  }
+  __device__ __forceinline__ float weight(const DistillArgs &a, int n) const {
+    return v[n] >= 0 ? __builtin_amdgcn_exp2f((t[n] - top) * a.c2) : 0.0f;
+  }
+};
+
+// U pieces in flight a thread; a piece past the end is loaded again from the last place and does not count
+template <typename T, int P, bool NT> __global__ __launch_bounds__(256) void distill_fwd_kernel(const DistillArgs a) {
   constexpr int E = Piece<T>::E, R = 256 / P, U = 4;
-  __shared__ float tps[R][kDistillMax], red[4];
-  __shared__ int64_t tis[R][kDistillMax];
-  const int t = threadIdx.x % P, rw = threadIdx.x / P;
-  const int64_t row = (int64_t)blockIdx.x * R + rw;
+  __shared__ float red[4];
+  const int t = threadIdx.x % P;
+  const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / P;
   if (P == 64 && row >= a.n) return;                       // (one wave a row: no barrier of the workgroup follows)
   const T *z = static_cast<const T *>(a.z) + row * a.stride;
-  const int off = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-  const int64_t pieces = (a.V + off + E - 1) / E;
+  const Cut<T> cut(z, (int)a.V);
+  Teacher<P> te;
+  te.load(a, row, t);
   float m = -__builtin_inff(), l = 0.0f;
-  for (int64_t i0 = t; i0 < pieces; i0 += (int64_t)P * U) {
-    float x[U][E];
+  auto take = [&](const float *x, int n) {
+    float top = m;
+    for (int e = 0; e < n; ++e) top = fmaxf(top, x[e]);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    l *= __builtin_amdgcn_exp2f((m - base) * a.c2);
+    for (int e = 0; e < n; ++e) l += power<T>(x[e], base, base * a.c2, a.c2);
+    m = top;
+  };
+  const uint4 *pieces = reinterpret_cast<const uint4 *>(z + cut.head);
+  uint4 u[U];
+  auto fetch = [&](int i0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) get_piece<T>(z, (i0 + (int64_t)u * P) * E - off, a.V, -__builtin_inff(), x[u]);
+    for (int n = 0; n < U; ++n) u[n] = load16<NT>(pieces + min(max(i0 + n * P, 0), cut.full - 1));
+  };
+  if (cut.full > 0) fetch(t - cut.skip);
+  te.gather(a, z);                                         // (behind the row's first pieces, before its lines are gone)
+  for (int i0 = t - cut.skip; i0 < cut.full; i0 += P * U) {
+    if (i0 != t - cut.skip) fetch(i0);
+    float x[U * E];
+#pragma unroll
+    for (int n = 0; n < U; ++n) {
+      float y[E];
+      widen<T>(u[n], y);
+      const bool in = i0 + n * P >= 0 && i0 + n * P < cut.full;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[n * E + e] = in ? y[e] : -__builtin_inff();
+    }
     float top = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) top = fmaxf(top, x[u][e]);
+    for (int e = 0; e < U * E; ++e) top = fmaxf(top, x[e]);
     const float base = top == -__builtin_inff() ? 0.0f : top;
     l *= __builtin_amdgcn_exp2f((m - base) * a.c2);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e) l += __builtin_amdgcn_exp2f((x[u][e] - base) * a.c2);
+    for (int e = 0; e < U * E; ++e) l += power<T>(x[e], base, base * a.c2, a.c2);
     m = top;
+  }
+  {                                                        // the ends of the row: fewer than E elements each
+    const int e = t < cut.head ? t : t - cut.head + cut.rest;
+    if (t < cut.head + (int)a.V - cut.rest) {
+      const float x = (float)z[e];
+      take(&x, 1);
+    }
   }
   const float M = row_max<P>(m, red), base = M == -__builtin_inff() ? 0.0f : M;
   const float L = row_sum<P>(l * __builtin_amdgcn_exp2f((m - base) * a.c2), red);
-  float top, mass;
-  const bool some = teacher_row<P>(a, row, t, tps[rw], tis[rw], red, top, mass);
+  const bool some = te.sum(a, red);
   float s = 0.0f;
   if (some) {
-    const float lm = logf(mass), lL = logf(L);
-    for (int j = t; j < a.k; j += P) {
-      const int64_t v = tis[rw][j];
-      if (v < 0) continue;
-      const float d = (tps[rw][j] - top) / a.T;
-      const float p = __builtin_amdgcn_exp2f((tps[rw][j] - top) * a.c2) / mass;
-      if (p != 0.0f) s += p * ((d - lm) - (((float)z[v] - base) / a.T - lL));
+    const float lm = logf(te.mass), lL = logf(L);
+#pragma unroll
+    for (int n = 0; n < Teacher<P>::N; ++n) {
+      if (te.v[n] < 0) continue;
+      const float p = te.weight(a, n) / te.mass;
+      if (p != 0.0f) s += p * (((te.t[n] - te.top) / a.T - lm) - ((te.z[n] - base) / a.T - lL));
     }
   }
   s = row_sum<P>(s, red);
@@ -158,72 +222,97 @@ template <typename T, int P> __global__ __launch_bounds__(256) void distill_fwd_
   }
 }
 
-template <typename T, int P> __global__ __launch_bounds__(256) void distill_bwd_kernel(const DistillArgs a) {
-  constexpr int E = Piece<T>::E, R = 256 / P, U = 2;
-  __shared__ float tps[R][kDistillMax], red[4];
-  __shared__ int64_t tis[R][kDistillMax];
+template <typename T, int P, bool NT> __global__ __launch_bounds__(256) void distill_bwd_kernel(const DistillArgs a) {
+  constexpr int E = Piece<T>::E, R = 256 / P, U = 4;
+  __shared__ float ws[R][kDistillMax], red[4];
+  __shared__ int vs[R][kDistillMax];
   const int t = threadIdx.x % P, rw = threadIdx.x / P;
   const int64_t row = (int64_t)blockIdx.x * R + rw;
   if (P == 64 && row >= a.n) return;
   const T *z = static_cast<const T *>(a.z) + row * a.stride;
   T *dz = static_cast<T *>(a.dz) + row * a.V;
-  const int off = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-  const bool vec = off == (int)((reinterpret_cast<uintptr_t>(dz) & 15) / sizeof(T));
-  const int64_t pieces = (a.V + off + E - 1) / E;
-  float top, mass;
-  const bool some = teacher_row<P>(a, row, t, tps[rw], tis[rw], red, top, mass);
-  const float w = a.g[row] * a.T;
-  const float base = a.stats[2 * row], f = some ? w / a.stats[2 * row + 1] : 0.0f;
-  for (int64_t i0 = t; i0 < pieces; i0 += (int64_t)P * U) {
-    float x[U][E];
+  const Cut<T> cut(z, (int)a.V);
+  const bool vec = (reinterpret_cast<uintptr_t>(dz + cut.head) & 15) == 0;
+  Teacher<P> te;
+  te.load(a, row, t);
+  const float w = a.g[row] * a.T, base = a.stats[2 * row], L = a.stats[2 * row + 1];
+  const float f = w / L;
+  const uint4 *pieces = reinterpret_cast<const uint4 *>(z + cut.head);
+  uint4 u[U];
+  auto fetch = [&](int i0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) get_piece<T>(z, (i0 + (int64_t)u * P) * E - off, a.V, 0.0f, x[u]);
+    for (int n = 0; n < U; ++n) u[n] = load16<NT>(pieces + min(max(i0 + n * P, 0), cut.full - 1));
+  };
+  if (cut.full > 0) fetch(t - cut.skip);
+  te.gather(a, z);
+  const bool some = te.sum(a, red);
+  const float base2 = base * a.c2;
+  auto grad = [&](float x) { return some ? f * power<T>(x, base, base2, a.c2) : 0.0f; };
+  for (int i0 = t - cut.skip; i0 < cut.full; i0 += P * U) {
+    if (i0 != t - cut.skip) fetch(i0);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t e0 = (i0 + (int64_t)u * P) * E - off;
+    for (int n = 0; n < U; ++n) {
+      if (i0 + n * P < 0 || i0 + n * P >= cut.full) continue;
+      float x[E];
+      widen<T>(u[n], x);
       T y[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = (T)(some ? f * __builtin_amdgcn_exp2f((x[u][e] - base) * a.c2) : 0.0f);
-      if (vec && e0 >= 0 && e0 + E <= a.V) {
-        uint4 o;
-        __builtin_memcpy(&o, y, 16);
-        *reinterpret_cast<uint4 *>(dz + e0) = o;
+      for (int e = 0; e < E; ++e) y[e] = (T)grad(x[e]);
+      T *o = dz + cut.head + (int64_t)(i0 + n * P) * E;
+      if (vec) {
+        uint4 q;
+        __builtin_memcpy(&q, y, 16);
+        // (past the caches: the gradient is as large as the logits, which the next pass wants there; 16 - 27 % of the
+        //  next forward's time at 206 and 308 MB)
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4nt, q), reinterpret_cast<u32x4nt *>(o));
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (e0 + e >= 0 && e0 + e < a.V) dz[e0 + e] = y[e];
+        for (int e = 0; e < E; ++e) o[e] = y[e];
       }
     }
   }
+  if (t < cut.head + (int)a.V - cut.rest) {
+    const int e = t < cut.head ? t : t - cut.head + cut.rest;
+    dz[e] = (T)grad((float)z[e]);
+  }
   if (!some) return;                                       // (the same for all threads of the row)
+#pragma unroll
+  for (int n = 0; n < Teacher<P>::N; ++n) {
+    const int j = t + n * P;
+    if (j < a.k) { ws[rw][j] = te.weight(a, n); vs[rw][j] = te.v[n]; }
+  }
   row_sync<P>();                                           // the row is written before its k places are written again
-  for (int j = t; j < a.k; j += P) {
-    const int64_t v = tis[rw][j];
+#pragma unroll
+  for (int n = 0; n < Teacher<P>::N; ++n) {
+    const int j = t + n * P, v = te.v[n];
     if (v < 0) continue;
     float p = 0.0f;
     bool first = true;
     for (int x = 0; x < a.k; ++x)
-      if (tis[rw][x] == v) {
-        if (x < j) first = false;
-        p += __builtin_amdgcn_exp2f((tps[rw][x] - top) * a.c2);
+      if (vs[rw][x] == v) {
+        first &= x >= j;
+        p += ws[rw][x];
       }
-    if (first) dz[v] = (T)(f * __builtin_amdgcn_exp2f(((float)z[v] - base) * a.c2) - w * (p / mass));
+    if (first) dz[v] = (T)(grad(te.z[n]) - w * (p / te.mass));
   }
 }
 
 // Rows of up to this many elements take a wave each, longer ones a workgroup.
-constexpr int64_t kDistillWaveRow = 2048;
+constexpr int64_t kDistillWaveRow = 16384;
+constexpr int64_t kDistillCache = (int64_t)256 << 20;      // bytes; see load16
+
+template <typename T, int P, bool NT> static void distill_launch(const DistillArgs &a, bool backward, hipStream_t s) {
+  const unsigned grid = (unsigned)((a.n + 256 / P - 1) / (256 / P));
+  if (backward) hipLaunchKernelGGL((distill_bwd_kernel<T, P, NT>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((distill_fwd_kernel<T, P, NT>), dim3(grid), dim3(256), 0, s, a);
+}
 
 template <typename T> static int distill_run(const DistillArgs &a, bool backward, hipStream_t s) {
-  const bool wave = a.V <= kDistillWaveRow;
-  const unsigned grid = (unsigned)(wave ? (a.n + 3) / 4 : a.n);
-  if (!backward) {
-    if (wave) hipLaunchKernelGGL((distill_fwd_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((distill_fwd_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
-  } else {
-    if (wave) hipLaunchKernelGGL((distill_bwd_kernel<T, 64>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3(grid), dim3(256), 0, s, a);
-  }
+  const bool wave = a.V <= kDistillWaveRow, stream = a.n * a.V * (int64_t)sizeof(T) > kDistillCache;
+  if (wave && stream) distill_launch<T, 64, true>(a, backward, s);
+  else if (wave) distill_launch<T, 64, false>(a, backward, s);
+  else if (stream) distill_launch<T, 256, true>(a, backward, s);
+  else distill_launch<T, 256, false>(a, backward, s);
   HSGK_LAUNCH_CHECK();
   return 0;
 }
