@@ -3,9 +3,11 @@
 // Per row: p = softmax over the k entries of t / T (an entry outside [0, V) or with t = -inf does not count),
 //   q = softmax over all V of z / T,   loss = T^2 sum_j p_j (log p_j - log q_{idx_j})   (no entry: 0)
 //   dz_v = g T (q_v - sum_{j: idx_j = v} p_j)                                            (no entry: 0)
-// Both passes are bound by memory: the forward reads the row once (running maximum and sum per thread, joined at the
-// end) and leaves (maximum, sum) for the backward, which reads the row and writes the gradient once; the k places
-// where p enters are written again at the end of the row, out of the cache, by one thread for each different index.
+// Both passes are bound by memory: the forward reads the row once and leaves (maximum, sum) for the backward, which reads
+// the row and writes the gradient once.  Rows that fit go through LDS (a wave each), longer ones through registers with a
+// running maximum and sum (a workgroup each).  TB/s of what has to move, where a 1 GiB copy reaches 5.2 (forward, backward):
+// 50176 x 4096 bfloat16, k = 32: 4.4, 5.4; 4099 (rows start anywhere): 3.9, 4.9; 37632 x 2048 float32, k = 20: 4.6, 5.7;
+// 12544 x 16384 bfloat16: 5.2, 5.7; 1031 x 100003 float16, k = 64: 3.4 (four workgroups a CU), 5.2.
 #include <math.h>
 
 #include "common.h"
@@ -145,15 +147,64 @@ template <int P> struct Teacher {
   __device__ __forceinline__ float weight(const DistillArgs &a, int n) const {
     return v[n] >= 0 ? __builtin_amdgcn_exp2f((t[n] - top) * a.c2) : 0.0f;
   }
+  // this thread's share of sum_j p_j (log p_j - log q_j)
+  __device__ __forceinline__ float loss(const DistillArgs &a, float base, float L) const {
+    const float lm = logf(mass), lL = logf(L);
+    float s = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (v[n] < 0) continue;
+      const float p = weight(a, n) / mass;
+      if (p != 0.0f) s += p * (((t[n] - top) / a.T - lm) - ((z[n] - base) / a.T - lL));
+    }
+    return s;
+  }
 };
 
-// U pieces in flight a thread; a piece past the end is loaded again from the last place and does not count
-template <typename T, int P, bool NT> __global__ __launch_bounds__(256) void distill_fwd_kernel(const DistillArgs a) {
-  constexpr int E = Piece<T>::E, R = 256 / P, U = 4;
+template <typename T> __device__ __forceinline__ void put_piece(T *o, const T (&y)[Piece<T>::E], bool vec) {
+  if (vec) {
+    uint4 q;
+    __builtin_memcpy(&q, y, 16);
+    // (past the caches: the gradient is as large as the logits, which the next pass wants there; 16 - 27 % of the
+    //  next forward's time at 206 and 308 MB)
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4nt, q), reinterpret_cast<u32x4nt *>(o));
+  } else {
+#pragma unroll
+    for (int e = 0; e < Piece<T>::E; ++e) o[e] = y[e];
+  }
+}
+
+// the row is written: its k places are written again, each different one by the first entry that names it
+template <typename T, int P, typename Grad>
+__device__ __forceinline__ void put_entries(const DistillArgs &a, const Teacher<P> &te, int t, float *ws, int *vs, float w, T *dz,
+                                            Grad grad) {
+#pragma unroll
+  for (int n = 0; n < Teacher<P>::N; ++n) {
+    const int j = t + n * P;
+    if (j < a.k) { ws[j] = te.weight(a, n); vs[j] = te.v[n]; }
+  }
+  row_sync<P>();
+#pragma unroll
+  for (int n = 0; n < Teacher<P>::N; ++n) {
+    const int j = t + n * P, v = te.v[n];
+    if (v < 0) continue;
+    float p = 0.0f;
+    bool first = true;
+    for (int x = 0; x < a.k; ++x)
+      if (vs[x] == v) {
+        first &= x >= j;
+        p += ws[x];
+      }
+    if (first) dz[v] = (T)(grad(te.z[n]) - w * (p / te.mass));
+  }
+}
+
+// Longer rows: a workgroup each, U pieces a thread at a time; a piece past the end is loaded again from the last place and does not count
+template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_fwd_kernel(const DistillArgs a) {
+  constexpr int P = 256, E = Piece<T>::E, U = 4;
   __shared__ float red[4];
-  const int t = threadIdx.x % P;
-  const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / P;
-  if (P == 64 && row >= a.n) return;                       // (one wave a row: no barrier of the workgroup follows)
+  const int t = threadIdx.x;
+  const int64_t row = blockIdx.x;
   const T *z = static_cast<const T *>(a.z) + row * a.stride;
   const Cut<T> cut(z, (int)a.V);
   Teacher<P> te;
@@ -205,30 +256,19 @@ template <typename T, int P, bool NT> __global__ __launch_bounds__(256) void dis
   const float M = row_max<P>(m, red), base = M == -__builtin_inff() ? 0.0f : M;
   const float L = row_sum<P>(l * __builtin_amdgcn_exp2f((m - base) * a.c2), red);
   const bool some = te.sum(a, red);
-  float s = 0.0f;
-  if (some) {
-    const float lm = logf(te.mass), lL = logf(L);
-#pragma unroll
-    for (int n = 0; n < Teacher<P>::N; ++n) {
-      if (te.v[n] < 0) continue;
-      const float p = te.weight(a, n) / te.mass;
-      if (p != 0.0f) s += p * (((te.t[n] - te.top) / a.T - lm) - ((te.z[n] - base) / a.T - lL));
-    }
-  }
-  s = row_sum<P>(s, red);
+  const float s = row_sum<P>(some ? te.loss(a, base, L) : 0.0f, red);
   if (t == 0) {
     a.loss[row] = some ? a.T * a.T * s : 0.0f;
     if (a.stats) { a.stats[2 * row] = base; a.stats[2 * row + 1] = L; }
   }
 }
 
-template <typename T, int P, bool NT> __global__ __launch_bounds__(256) void distill_bwd_kernel(const DistillArgs a) {
-  constexpr int E = Piece<T>::E, R = 256 / P, U = 4;
-  __shared__ float ws[R][kDistillMax], red[4];
-  __shared__ int vs[R][kDistillMax];
-  const int t = threadIdx.x % P, rw = threadIdx.x / P;
-  const int64_t row = (int64_t)blockIdx.x * R + rw;
-  if (P == 64 && row >= a.n) return;
+template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_bwd_kernel(const DistillArgs a) {
+  constexpr int P = 256, E = Piece<T>::E, U = 4;
+  __shared__ float ws[kDistillMax], red[4];
+  __shared__ int vs[kDistillMax];
+  const int t = threadIdx.x;
+  const int64_t row = blockIdx.x;
   const T *z = static_cast<const T *>(a.z) + row * a.stride;
   T *dz = static_cast<T *>(a.dz) + row * a.V;
   const Cut<T> cut(z, (int)a.V);
@@ -259,60 +299,157 @@ template <typename T, int P, bool NT> __global__ __launch_bounds__(256) void dis
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = (T)grad(x[e]);
       T *o = dz + cut.head + (int64_t)(i0 + n * P) * E;
-      if (vec) {
-        uint4 q;
-        __builtin_memcpy(&q, y, 16);
-        // (past the caches: the gradient is as large as the logits, which the next pass wants there; 16 - 27 % of the
-        //  next forward's time at 206 and 308 MB)
-        __builtin_nontemporal_store(__builtin_bit_cast(u32x4nt, q), reinterpret_cast<u32x4nt *>(o));
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = y[e];
-      }
+      put_piece<T>(o, y, vec);
     }
   }
   if (t < cut.head + (int)a.V - cut.rest) {
     const int e = t < cut.head ? t : t - cut.head + cut.rest;
     dz[e] = (T)grad((float)z[e]);
   }
-  if (!some) return;                                       // (the same for all threads of the row)
-#pragma unroll
-  for (int n = 0; n < Teacher<P>::N; ++n) {
-    const int j = t + n * P;
-    if (j < a.k) { ws[rw][j] = te.weight(a, n); vs[rw][j] = te.v[n]; }
+  if (some) put_entries<T, P>(a, te, t, ws, vs, w, dz, grad);        // (the same for all threads of the row)
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Rows that fit LDS: a wave each, R of them a workgroup.  The row comes straight into LDS, whole, past the registers, so its
+// length and not U bounds what is under way, and the teacher's k places are read there: in memory those reads touched
+// nearly half of a row's lines a second time.
+template <bool NT> __device__ __forceinline__ void row_to_lds(const void *from, uint32_t lds_byte) {
+  if (NT) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_byte), "v"(from) : "memory");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_byte), "v"(from) : "memory");
+}
+
+// bytes of LDS of a row: 128 in front (the head and the line's start), whole pieces, the rest
+template <typename T> constexpr int lds_row_bytes(int64_t V) { return 128 + (int)((V * (int64_t)sizeof(T) + 15) / 16 + 1) * 16; }
+
+// sends for the row; element e will lie at x[e] of the returned pointer
+template <typename T, bool NT>
+__device__ __forceinline__ T *fetch_row(const T *z, const Cut<T> &cut, int V, unsigned char *lds, int lane) {
+  constexpr int E = Piece<T>::E;
+  const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)(lds)) + 128;
+  T *x = reinterpret_cast<T *>(lds + 128) - cut.head;
+  for (int i0 = -cut.skip; i0 < cut.full; i0 += 64) {
+    const int i = i0 + lane;
+    if (i >= 0 && i < cut.full) row_to_lds<NT>(z + cut.head + (int64_t)i * E, __builtin_amdgcn_readfirstlane(base + (uint32_t)(i0 * 16)));
   }
-  row_sync<P>();                                           // the row is written before its k places are written again
+  if (lane < cut.head + V - cut.rest) {
+    const int e = lane < cut.head ? lane : lane - cut.head + cut.rest;
+    x[e] = z[e];
+  }
+  return x;
+}
+__device__ __forceinline__ void row_has_come() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);                      // vmcnt(0) lgkmcnt(0): the row and its ends
+  asm volatile("" ::: "memory");
+}
+
+template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_fwd_row_kernel(const DistillArgs a) {
+  constexpr int E = Piece<T>::E;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds_rows[];
+  const int t = threadIdx.x & 63, rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + rw;
+  if (row >= a.n) return;                                  // (no barrier of the workgroup follows)
+  const T *z = static_cast<const T *>(a.z) + row * a.stride;
+  const int V = (int)a.V;
+  const Cut<T> cut(z, V);
+  Teacher<64> te;
+  te.load(a, row, t);
+  const T *x = fetch_row<T, NT>(z, cut, V, lds_rows + rw * lds_row_bytes<T>(V), t);
+  row_has_come();
+  te.gather(a, x);
+  const bool end = t < cut.head + V - cut.rest;
+  const float xe = end ? (float)x[t < cut.head ? t : t - cut.head + cut.rest] : -__builtin_inff();
+  const uint4 *pieces = reinterpret_cast<const uint4 *>(x + cut.head);
+  float top = xe;
+  for (int i = t; i < cut.full; i += 64) {
+    float y[E];
+    widen<T>(pieces[i], y);
 #pragma unroll
-  for (int n = 0; n < Teacher<P>::N; ++n) {
-    const int j = t + n * P, v = te.v[n];
-    if (v < 0) continue;
-    float p = 0.0f;
-    bool first = true;
-    for (int x = 0; x < a.k; ++x)
-      if (vs[rw][x] == v) {
-        first &= x >= j;
-        p += ws[rw][x];
-      }
-    if (first) dz[v] = (T)(grad(te.z[n]) - w * (p / te.mass));
+    for (int e = 0; e < E; ++e) top = fmaxf(top, y[e]);
+  }
+  top = row_max<64>(top, nullptr);
+  const float base = top == -__builtin_inff() ? 0.0f : top, base2 = base * a.c2;
+  float l = end ? power<T>(xe, base, base2, a.c2) : 0.0f;
+  for (int i = t; i < cut.full; i += 64) {
+    float y[E];
+    widen<T>(pieces[i], y);
+#pragma unroll
+    for (int e = 0; e < E; ++e) l += power<T>(y[e], base, base2, a.c2);
+  }
+  const float L = row_sum<64>(l, nullptr);
+  const bool some = te.sum(a, nullptr);
+  const float s = row_sum<64>(some ? te.loss(a, base, L) : 0.0f, nullptr);
+  if (t == 0) {
+    a.loss[row] = some ? a.T * a.T * s : 0.0f;
+    if (a.stats) { a.stats[2 * row] = base; a.stats[2 * row + 1] = L; }
   }
 }
 
-// Rows of up to this many elements take a wave each, longer ones a workgroup.
-constexpr int64_t kDistillWaveRow = 16384;
+template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_bwd_row_kernel(const DistillArgs a) {
+  constexpr int E = Piece<T>::E;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds_rows[];
+  __shared__ float ws[4][kDistillMax];
+  __shared__ int vs[4][kDistillMax];
+  const int t = threadIdx.x & 63, rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + rw;
+  if (row >= a.n) return;
+  const T *z = static_cast<const T *>(a.z) + row * a.stride;
+  T *dz = static_cast<T *>(a.dz) + row * a.V;
+  const int V = (int)a.V;
+  const Cut<T> cut(z, V);
+  Teacher<64> te;
+  te.load(a, row, t);
+  const float w = a.g[row] * a.T, base = a.stats[2 * row], L = a.stats[2 * row + 1];
+  T *x = fetch_row<T, NT>(z, cut, V, lds_rows + rw * lds_row_bytes<T>(V), t);
+  row_has_come();
+  te.gather(a, x);
+  const bool some = te.sum(a, nullptr);
+  const float f = w / L, base2 = base * a.c2;
+  auto grad = [&](float v) { return some ? f * power<T>(v, base, base2, a.c2) : 0.0f; };
+  // the gradient takes the logits' place in LDS, its k places are corrected there, and it leaves in whole lines
+  uint4 *pieces = reinterpret_cast<uint4 *>(x + cut.head);
+  for (int i = t; i < cut.full; i += 64) {
+    float v[E];
+    widen<T>(pieces[i], v);
+    T y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = (T)grad(v[e]);
+    __builtin_memcpy(&pieces[i], y, 16);
+  }
+  const bool end = t < cut.head + V - cut.rest;
+  const int at = t < cut.head ? t : t - cut.head + cut.rest;
+  if (end) x[at] = (T)grad((float)x[at]);
+  if (some) put_entries<T, 64>(a, te, t, ws[rw], vs[rw], w, x, grad);
+  row_sync<64>();
+  const bool vec = (reinterpret_cast<uintptr_t>(dz + cut.head) & 15) == 0;
+  for (int i = t - cut.skip; i < cut.full; i += 64) {
+    if (i < 0) continue;
+    T y[E];
+    __builtin_memcpy(y, &pieces[i], 16);
+    put_piece<T>(dz + cut.head + (int64_t)i * E, y, vec);
+  }
+  if (end) dz[at] = x[at];
+}
+
+// Rows of up to kDistillRow bytes go through LDS, longer ones take a workgroup each and no LDS (forward + backward, us, LDS
+// and workgroup: 50176 rows of 8 KB 91 + 140 and 160 + 196; 12544 rows of 32 KB 145 + 184 and 81 + 156, too few waves fit).
+constexpr int64_t kDistillRow = 10 * 1024;
 constexpr int64_t kDistillCache = (int64_t)256 << 20;      // bytes; see load16
 
-template <typename T, int P, bool NT> static void distill_launch(const DistillArgs &a, bool backward, hipStream_t s) {
-  const unsigned grid = (unsigned)((a.n + 256 / P - 1) / (256 / P));
-  if (backward) hipLaunchKernelGGL((distill_bwd_kernel<T, P, NT>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((distill_fwd_kernel<T, P, NT>), dim3(grid), dim3(256), 0, s, a);
+template <typename T, bool NT> static void distill_launch(const DistillArgs &a, bool backward, hipStream_t s) {
+  if (a.V * (int64_t)sizeof(T) <= kDistillRow) {
+    const unsigned grid = (unsigned)((a.n + 3) / 4), lds = 4 * lds_row_bytes<T>(a.V);
+    if (backward) hipLaunchKernelGGL((distill_bwd_row_kernel<T, NT>), dim3(grid), dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((distill_fwd_row_kernel<T, NT>), dim3(grid), dim3(256), lds, s, a);
+  } else {
+    if (backward) hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)a.n), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((distill_fwd_kernel<T, NT>), dim3((unsigned)a.n), dim3(256), 0, s, a);
+  }
 }
 
 template <typename T> static int distill_run(const DistillArgs &a, bool backward, hipStream_t s) {
-  const bool wave = a.V <= kDistillWaveRow, stream = a.n * a.V * (int64_t)sizeof(T) > kDistillCache;
-  if (wave && stream) distill_launch<T, 64, true>(a, backward, s);
-  else if (wave) distill_launch<T, 64, false>(a, backward, s);
-  else if (stream) distill_launch<T, 256, true>(a, backward, s);
-  else distill_launch<T, 256, false>(a, backward, s);
+  if (a.n * a.V * (int64_t)sizeof(T) > kDistillCache) distill_launch<T, true>(a, backward, s);
+  else distill_launch<T, false>(a, backward, s);
   HSGK_LAUNCH_CHECK();
   return 0;
 }
