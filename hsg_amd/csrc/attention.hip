@@ -10,23 +10,25 @@ static int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 static int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
 struct AttnPlan {
-  bool shared;      // 32 columns a workgroup, its waves share them (else 128, 32 a wave)
-  int splits;       // parts of the streamed rows, joined by a second kernel
+  AttnShape shape;
+  int splits;          // parts of the streamed rows, joined by a second kernel
 };
 
 // Shared columns where 128 of them would leave CUs without a workgroup (float32, 28 heads x 131 queries x 203 keys, width
-// 36: forward 18 us on 126 shared workgroups; 192 heads x 256 x 256, width 32: 29 us on 384 of 128 columns, 40 on 1536
-// shared).  Split rows where there are fewer workgroups than `room`, what the CUs hold at a time: more only add partial
-// results (one token of 16 heads over 2 x 32768 keys, width 128: 256 workgroups 38 + 5 us, 512 42 + 5).  Causal blocks
-// differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys: 1345 us in one part, 773 + 32 in two).
-static AttnPlan attn_plan(const hsgk_attention_args &a, bool dkv) {
+// 36: forward, dq, dk and dv 16 + 17 + 25 us shared, 23 + 31 + 49 with 128; 192 heads x 256 x 256, width 32: 32 + 38 + 43
+// shared, 25 + 35 + 42 with 128).  Split rows where there are fewer workgroups than `room`, what the CUs hold at a time:
+// more only add partial results (one token of 16 heads over 2 x 32768 keys, width 128: 256 workgroups 25 + 4 us, 512
+// 30 + 4).  Causal blocks differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys: 1105 us in one
+// part, 760 + 16 in two).
+static AttnPlan attn_plan(const hsgk_attention_args &a, AttnPass pass) {
+  const bool dkv = pass == kAttnDkv;
   const int64_t heads = (int64_t)a.B * a.G, queries = (int64_t)a.L * (a.H / a.G);
   const int64_t columns = dkv ? a.S : queries, rows = dkv ? queries : a.S;
   const int bytes = padded_width(a.D) * elem_size(a.dtype);                 // of a row in LDS
   AttnPlan p;
-  p.shared = columns <= 32 || heads * ((columns + 127) / 128) < 256;
-  const int64_t per = p.shared ? 32 : 128, groups = heads * ((columns + per - 1) / per);
-  const bool alone = (p.shared && bytes >= 256) || (dkv && bytes >= 256);   // LDS or registers hold one workgroup a CU
+  p.shape = columns <= 32 || heads * ((columns + 127) / 128) < 256 ? kAttnShared : kAttnWide;
+  const int64_t per = p.shape == kAttnWide ? 128 : 32, groups = heads * ((columns + per - 1) / per);
+  const bool alone = (p.shape == kAttnShared && bytes >= 256) || (dkv && bytes >= 256);   // LDS or registers hold one workgroup a CU
   const int64_t room = alone && !a.causal ? 256 : 512;
   int64_t s = groups > 0 ? room / groups : 1;
   const int64_t most = rows / 256;
@@ -55,14 +57,14 @@ static AttnSpace attn_space(const hsgk_attention_args &a, bool backward, void *b
   AttnSpace w = {};
   const int64_t heads = (int64_t)a.B * a.G, C = (int64_t)a.L * (a.H / a.G);
   const size_t dp = (size_t)padded_width(a.D);
-  const AttnPlan f = attn_plan(a, false);
+  const AttnPlan f = attn_plan(a, backward ? kAttnDq : kAttnFwd);
   if (!backward) {
     if (f.splits > 1) {
       w.part = c.take<float>((size_t)f.splits * heads * C * dp);
       w.ml = c.take<float>((size_t)f.splits * heads * C * 2);
     }
   } else {
-    const AttnPlan r = attn_plan(a, true);
+    const AttnPlan r = attn_plan(a, kAttnDkv);
     const size_t n1 = f.splits > 1 ? (size_t)f.splits * heads * C * dp : 0;
     const size_t n2 = r.splits > 1 ? (size_t)r.splits * heads * a.S * dp : 0;
     w.delta = c.take<float>((size_t)heads * C);
@@ -155,10 +157,10 @@ static int attn_args(const hsgk_attention_args &p, const AttnSpace &w, bool back
   return 0;
 }
 
-static int attn_go(int dtype, AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s) {
+static int attn_go(int dtype, AttnPass pass, const AttnArgs &a, AttnShape shape, hipStream_t s) {
   if (pass == kAttnDkv)
-    return dtype == 0 ? attn_dkv_f32(pass, a, shared, s) : dtype == 1 ? attn_dkv_bf16(pass, a, shared, s) : attn_dkv_f16(pass, a, shared, s);
-  return dtype == 0 ? attn_f32(pass, a, shared, s) : dtype == 1 ? attn_bf16(pass, a, shared, s) : attn_f16(pass, a, shared, s);
+    return dtype == 0 ? attn_dkv_f32(pass, a, shape, s) : dtype == 1 ? attn_dkv_bf16(pass, a, shape, s) : attn_dkv_f16(pass, a, shape, s);
+  return dtype == 0 ? attn_f32(pass, a, shape, s) : dtype == 1 ? attn_bf16(pass, a, shape, s) : attn_f16(pass, a, shape, s);
 }
 
 }  // namespace hsgk
@@ -182,9 +184,9 @@ int hsgk_attention_fwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
   const AttnSpace w = attn_space(*args, false, args->workspace);
   AttnArgs a;
   if (int rc = attn_args(*args, w, false, s, a)) return rc;
-  const AttnPlan p = attn_plan(*args, false);
+  const AttnPlan p = attn_plan(*args, kAttnFwd);
   a.splits = p.splits; a.part = w.part; a.ml = w.ml; a.out = args->out;
-  return attn_go(args->dtype, kAttnFwd, a, p.shared, s);
+  return attn_go(args->dtype, kAttnFwd, a, p.shape, s);
 }
 
 int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
@@ -197,14 +199,14 @@ int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
   if (int rc = attn_args(*args, w, true, s, a)) return rc;
   a.delta = w.delta; a.part = w.part; a.part2 = w.part2;
   if (a.C > 0) {
-    const AttnPlan p = attn_plan(*args, false);
+    const AttnPlan p = attn_plan(*args, kAttnDq);
     a.splits = p.splits; a.out = args->dq;
-    if (int rc = attn_go(args->dtype, kAttnDq, a, p.shared, s)) return rc;
+    if (int rc = attn_go(args->dtype, kAttnDq, a, p.shape, s)) return rc;
   }
   if (a.S > 0 && args->dk) {
-    const AttnPlan p = attn_plan(*args, true);
+    const AttnPlan p = attn_plan(*args, kAttnDkv);
     a.splits = p.splits; a.out = args->dk; a.out2 = args->dv;
-    if (int rc = attn_go(args->dtype, kAttnDkv, a, p.shared, s)) return rc;
+    if (int rc = attn_go(args->dtype, kAttnDkv, a, p.shape, s)) return rc;
   }
   return 0;
 }

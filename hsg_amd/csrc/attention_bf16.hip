@@ -2,5 +2,5 @@
 #include "attention_tiles.h"
 
 namespace hsgk {
-HSGK_ATTN(attn_bf16) { return attn_type<__bf16, false>(pass, a, shared, s); }
+HSGK_ATTN(attn_bf16) { return attn_type<__bf16, false>(pass, a, shape, s); }
 }  // namespace hsgk

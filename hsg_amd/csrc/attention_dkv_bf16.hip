@@ -2,5 +2,5 @@
 #include "attention_tiles.h"
 
 namespace hsgk {
-HSGK_ATTN(attn_dkv_bf16) { return attn_type<__bf16, true>(pass, a, shared, s); }
+HSGK_ATTN(attn_dkv_bf16) { return attn_type<__bf16, true>(pass, a, shape, s); }
 }  // namespace hsgk

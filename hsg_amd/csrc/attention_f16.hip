@@ -2,5 +2,5 @@
 #include "attention_tiles.h"
 
 namespace hsgk {
-HSGK_ATTN(attn_f16) { return attn_type<_Float16, false>(pass, a, shared, s); }
+HSGK_ATTN(attn_f16) { return attn_type<_Float16, false>(pass, a, shape, s); }
 }  // namespace hsgk

@@ -2,5 +2,5 @@
 #include "attention_tiles.h"
 
 namespace hsgk {
-HSGK_ATTN(attn_f32) { return attn_type<float, false>(pass, a, shared, s); }
+HSGK_ATTN(attn_f32) { return attn_type<float, false>(pass, a, shape, s); }
 }  // namespace hsgk

@@ -247,7 +247,15 @@ __device__ __forceinline__ void load_columns(typename Tile<T, DP>::Columns &x, c
   }
 }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// maximum and sum over the two lanes that hold a column
+__device__ __forceinline__ float both_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float both_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
 
 __device__ __forceinline__ void col_of(const AttnArgs &a, int c, int &i, int &hh) {
   if (a.HG == 1) { i = c; hh = 0; } else { i = (int)((unsigned)c / (unsigned)a.HG); hh = c - i * a.HG; }
@@ -292,7 +300,7 @@ template <typename T, int DB> struct ColumnScale {
       float top = 0.0f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
-      top = fmaxf(top, other_half(top));
+      top = both_max(top);
       if (__any(top * f > 32768.0f)) {
         if (top * f > 32768.0f) {
           int e = 0;
@@ -321,7 +329,8 @@ template <typename T> constexpr float prob_shift() {         // log2 of the fact
 // tile's rows, their results joined at the end (KW = 4: few columns).
 // (Measured and not kept: 64 columns a wave, so that an A operand read from LDS serves two matrix instructions.  bfloat16,
 // us for 32, 64 and 2 x 64 columns with halved rows: forward of 16 heads x 8192 x 8192 causal, width 128, 435, 680, 901;
-// 96 heads x 785 x 785, width 64, 37, 46, 71.  One wave less a SIMD costs more than the LDS traffic.)
+// 96 heads x 785 x 785, width 64, 37, 46, 71.  One wave less a SIMD costs more than the LDS traffic.  Nor two waves for the
+// same 32 columns: 34 -> 47 and, 24 heads x 2305 x 2305, 60 -> 87.)
 template <typename T, int DP, int KW> struct Shape {
   static constexpr int COLS = 128 / KW;                                            // columns of a workgroup
   static constexpr int TR = KW == 4 ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64; // streamed rows per tile
@@ -330,6 +339,7 @@ template <typename T, int DP, int KW> struct Shape {
   static constexpr int NBUF = 4 * TILE <= 128 * 1024 ? 2 : 1;
   static constexpr int JOIN = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
   static constexpr int LDS = 2 * NBUF * TILE > JOIN ? 2 * NBUF * TILE : JOIN;
+  static constexpr bool UNROLL = sizeof(T) == 2;                                   // (float32: bound by its matrix instructions)
   static constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;                                            // see read_ahead
   // waves of a SIMD that the registers have to leave room for (no more than the LDS does)
   static constexpr int W0 = LDS > 80 * 1024 ? 1 : LDS > 52 * 1024 ? 2 : 3;
@@ -346,29 +356,41 @@ __device__ __forceinline__ void join_put(float *lds, const f32x16 (&acc)[DP / 32
 #pragma unroll
     for (int r = 0; r < 16; ++r) p[32 * db + 8 * (r >> 2) + (r & 3)] = acc[db][r] * f;
 }
-// element d of column col: the sum over the waves, in wave order
-template <int DP> __device__ __forceinline__ float join_get(const float *lds, int col, int d) {
-  const float *p = lds + col * (DP + 1) + d;
-  return ((p[0] + p[32 * (DP + 1)]) + p[2 * 32 * (DP + 1)]) + p[3 * 32 * (DP + 1)];
+// element d of column col: the sum over the waves that share it, in wave order
+template <int DP, int KW> __device__ __forceinline__ float join_get(const float *lds, int col, int d) {
+  const float *p = lds + ((col >> 5) * KW * 32 + (col & 31)) * (DP + 1) + d;
+  float s = p[0];
+#pragma unroll
+  for (int k = 1; k < KW; ++k) s += p[k * 32 * (DP + 1)];
+  return s;
 }
 
 // the tiles of [lo, hi), the first of which is on its way (issue(lo, 0)): the next one is while one is computed on.
 // land(buf): what a thread still does to its own share of the tile that has arrived, before the others see it.
-template <int TR, int NBUF, typename Issue, typename Land, typename Compute>
+template <int TR, int NBUF, bool UNROLL, typename Issue, typename Land, typename Compute>
 __device__ __forceinline__ void stream(int lo, int hi, Issue issue, Land land, Compute compute) {
-  int buf = 0;
-  for (int t0 = lo; t0 < hi; t0 += TR) {
+  auto step = [&](int t0, int buf) {
     const bool more = t0 + TR < hi;
     wait_for_lds();
     land(buf);
     __syncthreads();                          // the tile is whole, and nobody reads the other buffer any more
     if (NBUF == 2 && more) issue(t0 + TR, buf ^ 1);
     compute(t0, buf);
-    if (NBUF == 2) {
-      buf ^= 1;
-    } else if (more) {
+    if (NBUF == 1 && more) {
       __syncthreads();
       issue(t0 + TR, 0);
+    }
+  };
+  if (UNROLL && NBUF == 2) {                  // over the buffers, whose addresses are constants then: 4 - 8 % of the forward pass
+    for (int t0 = lo; t0 < hi; t0 += 2 * TR) {
+      step(t0, 0);
+      if (t0 + TR < hi) step(t0 + TR, 1);
+    }
+  } else {
+    int buf = 0;
+    for (int t0 = lo; t0 < hi; t0 += TR) {
+      step(t0, buf);
+      if (NBUF == 2) buf ^= 1;
     }
   }
   wait_for_lds();                             // (the first tile of an empty range)
@@ -382,9 +404,10 @@ template <int BYTES> __device__ __forceinline__ void clear_tiles(unsigned char *
 }
 
 // Which part, column block and (batch item, key head) a workgroup takes.  Workgroup ids are dealt round-robin over the 8
-// XCDs, each with an L2 of its own: workgroups that stream the same rows belong on one XCD.  Without causality consecutive
-// blocks of a head go to the same XCD; with it the blocks differ in work, so the longest of all heads come first and the
-// heads take turns (with 8 heads or a divisor or multiple of 8 a head still stays on its XCDs).  Parts of split rows are
+// XCDs, each with an L2 of its own: workgroups that stream the same rows belong on one XCD, and every XCD should get heads of
+// every batch item, whose lengths differ.  Without causality a head stays on one XCD, eight heads side by side.  With it the
+// blocks differ in work, so the longest of all heads come first and the heads take turns (with 8 heads or a divisor or
+// multiple of 8 a head still stays on its XCDs).  Parts of split rows are
 // counted from the end that every block sees, so the first parts are whole, and neighbours in the order differ little: within
 // an XCD workgroups are placed in order, and one that has to wait holds up the rest (dk and dv of 16 heads on 4, 8192 x 8192,
 // width 128: 1318 us with the two parts of a block next to each other, 857 this way).
@@ -402,12 +425,17 @@ __device__ __forceinline__ Place place_of(const AttnArgs &a, int blocks, bool de
     p.cb = (int)(id % (unsigned)blocks);
     if (descending) p.cb = blocks - 1 - p.cb;
   } else {
-    const unsigned n = gridDim.x, x = id & 7, per = n >> 3, rem = n & 7;
-    id = x * per + (x < rem ? x : rem) + (id >> 3);
+    const unsigned per = (unsigned)(blocks * a.splits), eights = (unsigned)(a.B * a.G) & ~7u;
+    if (id < eights * per) {
+      p.bg = (int)((id >> 3) / per * 8 + (id & 7));
+      id = (id >> 3) % per;
+    } else {
+      id -= eights * per;
+      p.bg = (int)(eights + id / per);
+      id %= per;
+    }
     p.sp = (int)(id % (unsigned)a.splits);
-    id /= (unsigned)a.splits;
-    p.cb = (int)(id % (unsigned)blocks);
-    p.bg = (int)(id / (unsigned)blocks);
+    p.cb = (int)(id / (unsigned)a.splits);
   }
   return p;
 }
@@ -451,8 +479,10 @@ __device__ inline int visible_end(const uint8_t *pad, int lo, int hi, int *red) 
 template <typename T, int DP, int TR> struct KeyRows {
   Rows<T, DP, TR> k, v;
   const T *kb, *vb;
-  uint32_t gone = 0;
-  int hidden = 0;
+  static constexpr int W = (TR + 63) / 64;
+  static_assert(W <= 2, "a tile's flags are two words");
+  int flag[W] = {}, left = 0;                           // of the tile on its way: row 64 i + lane is padded; rows up to the end
+  uint64_t gone[W] = {};                                // of the tile that has landed: the rows that nobody sees
   __device__ __forceinline__ void issue(const AttnArgs &a, const uint8_t *pad, int lo, int t0, int hi, const T *tk, const T *tv) {
     if (t0 == lo || t0 + TR > hi) {
       k.place([&](int j) { return kb + (int64_t)j * a.ks[1]; }, t0, hi);
@@ -463,27 +493,32 @@ template <typename T, int DP, int TR> struct KeyRows {
     }
     k.issue(tk, a.DL);
     v.issue(tv, a.DL);
-    const int j = t0 + (int)threadIdx.x;
-    hidden = j >= hi;
-    if (pad) {
-      gone = 0;
+    left = hi - t0;
+    if (pad) {                                          // (looked at only when the tile has landed: waiting here cost 40 %)
+#pragma unroll
+      for (int i = 0; i < W; ++i) flag[i] = pad[min(t0 + 64 * i + (int)(threadIdx.x & 63), hi - 1)];
+    }
+  }
+  __device__ __forceinline__ void land(bool pad, T *tk, T *tv) {
+    const int lane = (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int i = 0; i < W; ++i) gone[i] = __ballot(64 * i + lane < TR && (64 * i + lane >= left || flag[i]));
+    if (pad && any()) {                                 // (behind the end comes row end - 1, which may be padded)
+      uint32_t bits = 0;
 #pragma unroll
       for (int n = 0; n < Rows<T, DP, TR>::N; ++n) {
-        const int jn = t0 + Rows<T, DP, TR>::row_of(n);
-        if (jn >= hi || pad[jn]) gone |= 1u << n;   // (behind the end comes row end - 1, which may be padded)
+        const int row = Rows<T, DP, TR>::row_of(n);
+        bits |= (uint32_t)((word(row >> 6) >> (row & 63)) & 1) << n;
       }
-      if ((int)threadIdx.x < TR && j < hi) hidden = pad[j];
+      Rows<T, DP, TR>::clear(tk, bits);
+      Rows<T, DP, TR>::clear(tv, bits);
     }
   }
-  __device__ __forceinline__ void land(T *tk, T *tv, int *hid) const {
-    if (gone) {
-      Rows<T, DP, TR>::clear(tk, gone);
-      Rows<T, DP, TR>::clear(tv, gone);
-    }
-    if ((int)threadIdx.x < TR) hid[threadIdx.x] = hidden;
-  }
+  __device__ __forceinline__ uint64_t word(int i) const { return W == 1 || i == 0 ? gone[0] : gone[W - 1]; }
+  __device__ __forceinline__ bool any() const { return gone[0] || gone[W - 1]; }
+  // bit (r & 3) + 8 (r >> 2): the lane's row r of the 32 rows from r0 on
+  __device__ __forceinline__ uint32_t bits_of(int r0, int h) const { return (uint32_t)(word(r0 >> 6) >> ((r0 & 63) + 4 * h)); }
 };
-
 // ---------------------------------------------------------------------------------------------------------------------
 // forward: columns = queries, keys and values stream
 template <typename T, int DP, int KW>
@@ -493,13 +528,12 @@ void attn_fwd_kernel(const AttnArgs a) {
   using Ti = Tile<T, DP>;
   constexpr int TR = Sh::TR, NS = Sh::NS;
   __shared__ __attribute__((aligned(16))) unsigned char lds[Sh::LDS];
-  __shared__ __attribute__((aligned(16))) int hid[Sh::NBUF][TR];
   __shared__ float stat[2][4][32];
   __shared__ int red[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
   const Place at = place_of(a, (a.C + Sh::COLS - 1) / Sh::COLS, true);
   const int b = at.bg / a.G, gh = at.bg - b * a.G;
-  const int c0 = at.cb * Sh::COLS, c = c0 + (KW == 1 ? 32 * w : 0) + (lane & 31);
+  const int c0 = at.cb * Sh::COLS, c = c0 + 32 * (w / KW) + (lane & 31);
   const uint8_t *pad = a.pad ? a.pad + (int64_t)b * a.pad_b : nullptr;
   int lo, hi, first_limit;
   key_range(a, at.sp, TR, c0, Sh::COLS, lo, hi, first_limit);
@@ -525,42 +559,41 @@ void attn_fwd_kernel(const AttnArgs a) {
 #pragma unroll
   for (int db = 0; db < Ti::DB; ++db) acc[db] = f32x16{0.0f};
   float m = -__builtin_inff(), l = 0.0f;                              // maximum of the scores, this half's sum
-  auto compute = [&](int t0, int buf) {
+  constexpr int X = NS < 2 ? NS : 2;                                  // row blocks at a time
+  auto block = [&](int t0, int buf, int r0) {
     const T *tk = tile(buf, 0), *tv = tile(buf, 1);
-    const int r0 = KW == 1 ? 0 : 32 * NS * w;
-    float s[NS][16];
+    float s[X][16];
 #pragma unroll
-    for (int x = 0; x < NS; ++x) {
+    for (int x = 0; x < X; ++x) {
       f32x16 y = f32x16{0.0f};
 #pragma unroll
       for (int kk = 0; kk < Ti::KK; ++kk) mma(y, ln.rows(tk, r0 + 32 * x, kk), q[kk], T());
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[x][r] = y[r];
     }
-    read_ahead<NS * Ti::KK, NS * Ti::KK * Elem<T>::MMA, Sh::AHEAD>();
+    read_ahead<X * Ti::KK, X * Ti::KK * Elem<T>::MMA, Sh::AHEAD>();
     uint4 fv[Ti::DB];
 #pragma unroll
     for (int db = 0; db < Ti::DB; ++db) fv[db] = ln.cols(tv, r0, db, 0);
-    if (pad || t0 + TR > hi || t0 + TR - 1 > first_limit) {
+    if (st.any() || t0 + TR - 1 > first_limit) {
       rare();
 #pragma unroll
-      for (int x = 0; x < NS; ++x)
+      for (int x = 0; x < X; ++x) {
+        const uint32_t bits = st.bits_of(r0 + 32 * x, h);
+        const int row = t0 + r0 + 32 * x + 4 * h;
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int row = r0 + 32 * x + 8 * r4 + 4 * h;
-          const int4 hv = *reinterpret_cast<const int4 *>(&hid[buf][row]);
-          const int hx[4] = {hv.x, hv.y, hv.z, hv.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hx[e] || t0 + row + e > lim) s[x][4 * r4 + e] = -__builtin_inff();
+        for (int r = 0; r < 16; ++r) {
+          const int off = (r & 3) + 8 * (r >> 2);
+          if (((bits >> off) & 1) || row + off > lim) s[x][r] = -__builtin_inff();
         }
+      }
     }
     float top = s[0][0];
 #pragma unroll
-    for (int x = 0; x < NS; ++x)
+    for (int x = 0; x < X; ++x)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[x][r]);
-    top = fmaxf(top, other_half(top));
+    top = both_max(top);
     const float mn = fmaxf(m, top);
     if (__any(mn > m)) {                                              // (a column whose maximum stays: factor 1)
       const float f = mn > m ? exp2f((m - mn) * a.c2) : 1.0f;
@@ -573,14 +606,14 @@ void attn_fwd_kernel(const AttnArgs a) {
     }
     const float base = m == -__builtin_inff() ? 0.0f : prob_shift<T>() - m * a.c2;
 #pragma unroll
-    for (int x = 0; x < NS; ++x)
+    for (int x = 0; x < X; ++x)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[x][r] = __builtin_amdgcn_exp2f(fmaf(s[x][r], a.c2, base));
         l += s[x][r];
       }
 #pragma unroll
-    for (int x = 0; x < NS; ++x)
+    for (int x = 0; x < X; ++x)
 #pragma unroll
       for (int kk = 0; kk < Ti::RK; ++kk) {
         const uint4 p = row_frag<T>(s[x], kk);
@@ -588,13 +621,17 @@ void attn_fwd_kernel(const AttnArgs a) {
 #pragma unroll
         for (int db = 0; db < Ti::DB; ++db) {
           mma(acc[db], fv[db], p, T());
-          if (next < NS * Ti::RK) fv[db] = ln.cols(tv, r0 + 32 * (next / Ti::RK), db, next % Ti::RK);
+          if (next < X * Ti::RK) fv[db] = ln.cols(tv, r0 + 32 * (next / Ti::RK), db, next % Ti::RK);
         }
       }
   };
-  stream<TR, Sh::NBUF>(lo, hi, issue, [&](int buf) { st.land(tile(buf, 0), tile(buf, 1), hid[buf]); }, compute);
+  auto compute = [&](int t0, int buf) {
+#pragma unroll 1
+    for (int x = 0; x < NS; x += X) block(t0, buf, 32 * (NS * (w % KW) + x));
+  };
+  stream<TR, Sh::NBUF, Sh::UNROLL>(lo, hi, issue, [&](int buf) { st.land(pad, tile(buf, 0), tile(buf, 1)); }, compute);
 
-  l += other_half(l);
+  l = both_sum(l);
   const float mt = l == 0.0f ? -__builtin_inff() : m * a.c2 - prob_shift<T>();       // log2 of the factor taken out of l and acc
   auto out_row = [&](int ci, int ch) { return static_cast<T *>(a.out) + (((int64_t)b * a.L + ci) * a.H + gh * a.HG + ch) * a.D; };
   const int64_t first = (int64_t)at.bg * a.C, part = (int64_t)at.sp * a.B * a.G * a.C;
@@ -603,19 +640,24 @@ void attn_fwd_kernel(const AttnArgs a) {
     __syncthreads();
     if (h == 0) { stat[0][w][lane] = mt; stat[1][w][lane] = l; }
     __syncthreads();
-    auto top = [&](int col) { return fmaxf(fmaxf(stat[0][0][col], stat[0][1][col]), fmaxf(stat[0][2][col], stat[0][3][col])); };
-    const float M = top(lane & 31);
+    auto top = [&](int w0, int col) {                                 // over the waves that share the column
+      float x = stat[0][w0][col];
+#pragma unroll
+      for (int k = 1; k < KW; ++k) x = fmaxf(x, stat[0][w0 + k][col]);
+      return x;
+    };
+    const float M = top(w / KW * KW, lane & 31);
     join_put<DP>(jo, acc, exp2f(mt - (M == -__builtin_inff() ? 0.0f : M)), w, lane);
     __syncthreads();
-    for (int t = threadIdx.x; t < 32 * DP; t += 256) {
-      const int col = t / DP, d = t % DP, cc = c0 + col;
+    for (int t = threadIdx.x; t < Sh::COLS * DP; t += 256) {
+      const int col = t / DP, d = t % DP, cc = c0 + col, w0 = (col >> 5) * KW;
       if (cc >= a.C) continue;
-      float MM = top(col), L = 0.0f;
+      float MM = top(w0, col & 31), L = 0.0f;
       const bool none = MM == -__builtin_inff();
       if (none) MM = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) L += stat[1][k][col] * exp2f(stat[0][k][col] - MM);
-      const float o = join_get<DP>(jo, col, d);
+      for (int k = 0; k < KW; ++k) L += stat[1][w0 + k][col & 31] * exp2f(stat[0][w0 + k][col & 31] - MM);
+      const float o = join_get<DP, KW>(jo, col, d);
       if (a.splits > 1) {
         a.part[(part + first + cc) * DP + d] = o;
         if (d == 0) { a.ml[2 * (part + first + cc)] = none ? -__builtin_inff() : MM; a.ml[2 * (part + first + cc) + 1] = L; }
@@ -684,12 +726,11 @@ void attn_dq_kernel(const AttnArgs a) {
   using Ti = Tile<T, DP>;
   constexpr int TR = Sh::TR, NS = Sh::NS;
   __shared__ __attribute__((aligned(16))) unsigned char lds[Sh::LDS];
-  __shared__ __attribute__((aligned(16))) int hid[Sh::NBUF][TR];
   __shared__ int red[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
   const Place at = place_of(a, (a.C + Sh::COLS - 1) / Sh::COLS, true);
   const int b = at.bg / a.G, gh = at.bg - b * a.G;
-  const int c0 = at.cb * Sh::COLS, c = c0 + (KW == 1 ? 32 * w : 0) + (lane & 31);
+  const int c0 = at.cb * Sh::COLS, c = c0 + 32 * (w / KW) + (lane & 31);
   const bool mine = c < a.C;
   const uint8_t *pad = a.pad ? a.pad + (int64_t)b * a.pad_b : nullptr;
   int lo, hi, first_limit;
@@ -720,9 +761,9 @@ void attn_dq_kernel(const AttnArgs a) {
     for (int kk = 0; kk < Ti::KK; ++kk)
       delta += dot_piece<T>(g[kk], load_piece<T>(orow, kk * Elem<T>::KS + h * (Elem<T>::KS / 2), a.D, a.ovec));
   }
-  delta += other_half(delta);
+  delta = both_sum(delta);
   const float lse = mine ? a.lse[col_at] : __builtin_inff();
-  if (mine && h == 0 && at.sp == 0 && (KW == 1 || w == 0)) a.delta[col_at] = delta;
+  if (mine && h == 0 && at.sp == 0 && w % KW == 0) a.delta[col_at] = delta;
   if (pad && lo < hi) hi = visible_end(pad, lo, hi, red);
 
   f32x16 acc[Ti::DB];
@@ -732,10 +773,10 @@ void attn_dq_kernel(const AttnArgs a) {
   cs.start();
   auto compute = [&](int t0, int buf) {
     const T *tk = tile(buf, 0), *tv = tile(buf, 1);
-    const bool some_hidden = pad || t0 + TR > hi || t0 + TR - 1 > first_limit;
+    const bool some_hidden = st.any() || t0 + TR - 1 > first_limit;
 #pragma unroll 1
     for (int n = 0; n < NS; ++n) {
-      const int r0 = 32 * ((KW == 1 ? 0 : NS * w) + n);
+      const int r0 = 32 * (NS * (w % KW) + n);
       f32x16 x = f32x16{0.0f}, y = f32x16{0.0f};
 #pragma unroll
       for (int kk = 0; kk < Ti::KK; ++kk) {
@@ -751,14 +792,13 @@ void attn_dq_kernel(const AttnArgs a) {
       for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(x[r], a.c2, -lse)) * (y[r] - delta);
       if (some_hidden) {
         rare();
+        const uint32_t bits = st.bits_of(r0, h);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int row = r0 + 8 * r4 + 4 * h;
-          const int4 hv = *reinterpret_cast<const int4 *>(&hid[buf][row]);
-          const int hx[4] = {hv.x, hv.y, hv.z, hv.w};
+          const int row = 8 * r4 + 4 * h;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (hx[e] || t0 + row + e > lim) ds[4 * r4 + e] = 0.0f;
+            if (((bits >> (8 * r4 + e)) & 1) || t0 + r0 + row + e > lim) ds[4 * r4 + e] = 0.0f;
         }
       }
       cs.apply(ds, acc);
@@ -773,7 +813,7 @@ void attn_dq_kernel(const AttnArgs a) {
       }
     }
   };
-  stream<TR, Sh::NBUF>(lo, hi, issue, [&](int buf) { st.land(tile(buf, 0), tile(buf, 1), hid[buf]); }, compute);
+  stream<TR, Sh::NBUF, Sh::UNROLL>(lo, hi, issue, [&](int buf) { st.land(pad, tile(buf, 0), tile(buf, 1)); }, compute);
 
   const float f = a.scale / cs.f;
   const int64_t part = (int64_t)at.sp * a.B * a.G * a.C;
@@ -782,10 +822,10 @@ void attn_dq_kernel(const AttnArgs a) {
     __syncthreads();
     join_put<DP>(jo, acc, f, w, lane);
     __syncthreads();
-    for (int t = threadIdx.x; t < 32 * DP; t += 256) {
+    for (int t = threadIdx.x; t < Sh::COLS * DP; t += 256) {
       const int col = t / DP, d = t % DP, cc = c0 + col;
       if (cc >= a.C || d >= a.D) continue;
-      const float o = join_get<DP>(jo, col, d);
+      const float o = join_get<DP, KW>(jo, col, d);
       int ci, ch;
       col_of(a, cc, ci, ch);
       if (a.splits > 1) a.part[(part + (int64_t)at.bg * a.C + cc) * DP + d] = o;
@@ -812,7 +852,7 @@ void attn_dkv_kernel(const AttnArgs a) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
   const Place at = place_of(a, (a.S + Sh::COLS - 1) / Sh::COLS, false);          // (the first keys are seen by the most queries)
   const int b = at.bg / a.G, gh = at.bg - b * a.G;
-  const int j0 = at.cb * Sh::COLS, j = j0 + (KW == 1 ? 32 * w : 0) + (lane & 31);
+  const int j0 = at.cb * Sh::COLS, j = j0 + 32 * (w / KW) + (lane & 31);
   const bool mine = j < a.S, seen = mine && !(a.pad && a.pad[(int64_t)b * a.pad_b + j]);
   // columns (queries) of this workgroup
   int lo = 0, hi = a.C;
@@ -875,7 +915,7 @@ void attn_dkv_kernel(const AttnArgs a) {
     const bool some_hidden = a.causal && j0 + Sh::COLS - 1 > il + a.S - a.L;
 #pragma unroll 1
     for (int n = 0; n < NS; ++n) {
-      const int r0 = 32 * ((KW == 1 ? 0 : NS * w) + n);
+      const int r0 = 32 * (NS * (w % KW) + n);
       f32x16 x = f32x16{0.0f}, y = f32x16{0.0f};
 #pragma unroll
       for (int kk = 0; kk < Ti::KK; ++kk) {
@@ -928,7 +968,7 @@ void attn_dkv_kernel(const AttnArgs a) {
       }
     }
   };
-  stream<TR, Sh::NBUF>(
+  stream<TR, Sh::NBUF, Sh::UNROLL>(
       lo, hi, issue,
       [&](int buf) {
         if ((int)threadIdx.x < TR) { slse[buf][threadIdx.x] = rl; sdel[buf][threadIdx.x] = rd; slim[buf][threadIdx.x] = rlim; }
@@ -949,10 +989,10 @@ void attn_dkv_kernel(const AttnArgs a) {
       __syncthreads();
       join_put<DP>(jo, which ? av : ak, which ? fv : fk, w, lane);
       __syncthreads();
-      for (int t = threadIdx.x; t < 32 * DP; t += 256) {
+      for (int t = threadIdx.x; t < Sh::COLS * DP; t += 256) {
         const int col = t / DP, d = t % DP, jj = j0 + col;
         if (jj >= a.S || d >= a.D) continue;
-        const float o = join_get<DP>(jo, col, d);
+        const float o = join_get<DP, KW>(jo, col, d);
         if (a.splits > 1) (which ? a.part2 : a.part)[(part + jj) * DP + d] = o;
         else static_cast<T *>(which ? a.out2 : a.out)[(((int64_t)b * a.S + jj) * a.G + gh) * a.D + d] = (T)o;
       }
@@ -975,13 +1015,21 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_sum_kernel(const float *part, int splits, int B, int G, int n, int per, int D,
                                                        T *out) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)B * G * n;
-  const int64_t at = t / DP;
-  const int d = (int)(t % DP);
+  const int64_t at = t / (DP / 4);
+  const int d = (int)(t % (DP / 4)) * 4;
   if (at >= rows || d >= D) return;
-  float s = 0.0f;
-  for (int x = 0; x < splits; ++x) s += part[(x * rows + at) * DP + d];
+  f32x4v s = f32x4v{0.0f};
+  for (int x = 0; x < splits; ++x) s += *reinterpret_cast<const f32x4v *>(part + (x * rows + at) * DP + d);
   const int bg = (int)(at / n), c = (int)(at % n), b = bg / G, gh = bg % G;
-  out[((((int64_t)b * (n / per) + c / per) * G + gh) * per + c % per) * D + d] = (T)s;
+  T *to = out + ((((int64_t)b * (n / per) + c / per) * G + gh) * per + c % per) * D + d;
+  if (D % 4 == 0) {
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)s[e];
+    __builtin_memcpy(__builtin_assume_aligned(to, 4 * sizeof(T)), y, sizeof(y));
+  } else {
+    for (int e = 0; e < 4 && d + e < D; ++e) to[e] = (T)s[e];
+  }
 }
 
 // rows whose 16-byte pieces are not aligned, copied into aligned ones of DL elements (zeros past D): [B, n, heads, DL]
@@ -998,6 +1046,8 @@ __global__ __launch_bounds__(256) void attn_pack_kernel(const T *from, int64_t s
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
 enum AttnPass { kAttnFwd, kAttnDq, kAttnDkv };
+// columns of a workgroup: 32 that its waves share, or 128
+enum AttnShape { kAttnShared, kAttnWide };
 
 template <typename T, int DP, int KW, bool DKV> void attn_launch(AttnPass pass, const AttnArgs &a, hipStream_t s) {
   const int cols = DKV ? a.S : a.C, per = Shape<T, DP, KW>::COLS;
@@ -1011,14 +1061,14 @@ template <typename T, int DP, int KW, bool DKV> void attn_launch(AttnPass pass, 
   }
 }
 
-template <typename T, int DP, bool DKV> int attn_run(AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s) {
-  if (shared) attn_launch<T, DP, 4, DKV>(pass, a, s);
-  else attn_launch<T, DP, 1, DKV>(pass, a, s);
+template <typename T, int DP, bool DKV> int attn_run(AttnPass pass, const AttnArgs &a, AttnShape shape, hipStream_t s) {
+  if (shape == kAttnWide) attn_launch<T, DP, 1, DKV>(pass, a, s);
+  else attn_launch<T, DP, 4, DKV>(pass, a, s);
   HSGK_LAUNCH_CHECK();
   if (a.splits > 1) {
     const int n = DKV ? a.S : a.C, per = DKV ? 1 : a.HG;
     const int64_t rows = (int64_t)a.B * a.G * n;
-    const unsigned grid = (unsigned)((rows * DP + 255) / 256);
+    const unsigned grid = (unsigned)((rows * (DP / 4) + 255) / 256);
     if (pass == kAttnFwd)
       hipLaunchKernelGGL((attn_fwd_join_kernel<T, DP>), dim3((unsigned)rows), dim3(256), 0, s, a);
     else
@@ -1032,14 +1082,14 @@ template <typename T, int DP, bool DKV> int attn_run(AttnPass pass, const AttnAr
   return 0;
 }
 
-template <typename T, bool DKV> int attn_type(AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s) {
-  if (a.D <= 32) return attn_run<T, 32, DKV>(pass, a, shared, s);
-  if (a.D <= 64) return attn_run<T, 64, DKV>(pass, a, shared, s);
-  return attn_run<T, 128, DKV>(pass, a, shared, s);
+template <typename T, bool DKV> int attn_type(AttnPass pass, const AttnArgs &a, AttnShape shape, hipStream_t s) {
+  if (a.D <= 32) return attn_run<T, 32, DKV>(pass, a, shape, s);
+  if (a.D <= 64) return attn_run<T, 64, DKV>(pass, a, shape, s);
+  return attn_run<T, 128, DKV>(pass, a, shape, s);
 }
 
 // one translation unit a type and side, so that they build next to each other
-#define HSGK_ATTN(name) int name(AttnPass pass, const AttnArgs &a, bool shared, hipStream_t s)
+#define HSGK_ATTN(name) int name(AttnPass pass, const AttnArgs &a, AttnShape shape, hipStream_t s)
 HSGK_ATTN(attn_f32);
 HSGK_ATTN(attn_bf16);
 HSGK_ATTN(attn_f16);
