@@ -42,6 +42,7 @@ struct AttnArgs {
   void *out;                             // o, or dq, or dk (contiguous)
   void *out2;                            // dv
   float *lse, *delta;                    // [B,G,C]
+  int have_delta;                        // whose delta is there before dq: 0 nobody's, 1 everyone's, 2 see attn_dq_kernel
   float *part, *part2, *ml;              // split work: partial sums [splits][B*G][columns][DP], (m, l) [splits][B*G][C][2]
   int splits;
 };
@@ -718,8 +719,16 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_jo
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dq (and delta): columns = queries, keys and values stream
-template <typename T, int DP, int KW>
+// dq, or with SUM delta alone: columns = queries, keys and values stream
+//
+// delta = do . o carries the rounding of a 16-bit o: as much as one of do . v, while what is left of dp - delta over few
+// keys is no more (relative error of dq against 64 bits, where rounding the exact dq gives 1: 2.3 for 2 keys, 1.55 for 16,
+// 1.46 for 128, more where values have a common part).  Queries that see at most kAttnExactKeys keys therefore get delta =
+// sum p dp, summed in float32 by a launch of its own, whose two products they can afford (1.42 for every length; 96 heads
+// x 197 x 197, width 64, bfloat16: 11 us beside 12 + 14 + 15 for forward, dq, dk and dv).
+constexpr int kAttnExactKeys = 256;
+
+template <typename T, int DP, int KW, bool SUM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))
 void attn_dq_kernel(const AttnArgs a) {
   using Sh = Shape<T, DP, KW>;
@@ -727,6 +736,7 @@ void attn_dq_kernel(const AttnArgs a) {
   constexpr int TR = Sh::TR, NS = Sh::NS;
   __shared__ __attribute__((aligned(16))) unsigned char lds[Sh::LDS];
   __shared__ int red[4];
+  __shared__ float dsum[SUM && KW > 1 ? 4 : 1][32];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
   const Place at = place_of(a, (a.C + Sh::COLS - 1) / Sh::COLS, true);
   const int b = at.bg / a.G, gh = at.bg - b * a.G;
@@ -735,6 +745,10 @@ void attn_dq_kernel(const AttnArgs a) {
   const uint8_t *pad = a.pad ? a.pad + (int64_t)b * a.pad_b : nullptr;
   int lo, hi, first_limit;
   key_range(a, at.sp, TR, c0, Sh::COLS, lo, hi, first_limit);
+  int last, last_h;                                                   // 2: whose last query sees few keys, whatever the split
+  col_of(a, min(c0 + Sh::COLS, a.C) - 1, last, last_h);
+  const bool there = a.have_delta == 1 || (a.have_delta == 2 && last + a.S - a.L < kAttnExactKeys);
+  if (SUM && !there) return;
   auto tile = [&](int buf, int which) { return reinterpret_cast<T *>(lds + (2 * buf + which) * Sh::TILE); };
   clear_tiles<2 * Sh::NBUF * Sh::TILE>(lds, a.DL < DP);
   KeyRows<T, DP, TR> st;
@@ -754,17 +768,27 @@ void attn_dq_kernel(const AttnArgs a) {
                               : nullptr, a.DL, lane);
   const int64_t row_at = (((int64_t)b * a.L + i) * a.H + head) * a.D, col_at = (int64_t)at.bg * a.C + c;
   const int lim = a.causal ? i + a.S - a.L : a.S;
-  float delta = 0.0f;
-  if (mine) {
-    const T *orow = static_cast<const T *>(a.o) + row_at;
-#pragma unroll
-    for (int kk = 0; kk < Ti::KK; ++kk)
-      delta += dot_piece<T>(g[kk], load_piece<T>(orow, kk * Elem<T>::KS + h * (Elem<T>::KS / 2), a.D, a.ovec));
-  }
-  delta = both_sum(delta);
   const float lse = mine ? a.lse[col_at] : __builtin_inff();
-  if (mine && h == 0 && at.sp == 0 && w % KW == 0) a.delta[col_at] = delta;
   if (pad && lo < hi) hi = visible_end(pad, lo, hi, red);
+  const bool exact = SUM && hi - lo <= kAttnExactKeys;
+  float delta = 0.0f;
+  if (!SUM && there) {
+    if (mine) delta = a.delta[col_at];
+  } else if (!exact) {
+    if (mine) {
+      const T *orow = static_cast<const T *>(a.o) + row_at;
+#pragma unroll
+      for (int kk = 0; kk < Ti::KK; ++kk)
+        delta += dot_piece<T>(g[kk], load_piece<T>(orow, kk * Elem<T>::KS + h * (Elem<T>::KS / 2), a.D, a.ovec));
+    }
+    delta = both_sum(delta);
+    if (mine && h == 0 && at.sp == 0 && w % KW == 0) a.delta[col_at] = delta;
+    if (SUM) {
+      wait_for_lds();                                                 // (the first tile is on its way)
+      return;
+    }
+  }
+  float sum = 0.0f;
 
   f32x16 acc[Ti::DB];
 #pragma unroll
@@ -801,6 +825,11 @@ void attn_dq_kernel(const AttnArgs a) {
             if (((bits >> (8 * r4 + e)) & 1) || t0 + r0 + row + e > lim) ds[4 * r4 + e] = 0.0f;
         }
       }
+      if constexpr (SUM) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += ds[r];
+        continue;
+      }
       cs.apply(ds, acc);
 #pragma unroll
       for (int kk = 0; kk < Ti::RK; ++kk) {
@@ -814,6 +843,16 @@ void attn_dq_kernel(const AttnArgs a) {
     }
   };
   stream<TR, Sh::NBUF, Sh::UNROLL>(lo, hi, issue, [&](int buf) { st.land(pad, tile(buf, 0), tile(buf, 1)); }, compute);
+  if constexpr (SUM) {
+    delta = both_sum(sum);
+    if constexpr (KW > 1) {
+      if (h == 0) dsum[w][lane] = delta;
+      __syncthreads();
+      delta = (dsum[0][lane & 31] + dsum[1][lane & 31]) + (dsum[2][lane & 31] + dsum[3][lane & 31]);
+    }
+    if (mine && h == 0 && w % KW == 0) a.delta[col_at] = delta;
+    return;
+  }
 
   const float f = a.scale / cs.f;
   const int64_t part = (int64_t)at.sp * a.B * a.G * a.C;
@@ -1045,7 +1084,7 @@ __global__ __launch_bounds__(256) void attn_pack_kernel(const T *from, int64_t s
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
-enum AttnPass { kAttnFwd, kAttnDq, kAttnDkv };
+enum AttnPass { kAttnFwd, kAttnDelta, kAttnDq, kAttnDkv };
 // columns of a workgroup: 32 that its waves share, or 128
 enum AttnShape { kAttnShared, kAttnWide };
 
@@ -1056,8 +1095,10 @@ template <typename T, int DP, int KW, bool DKV> void attn_launch(AttnPass pass, 
     hipLaunchKernelGGL((attn_dkv_kernel<T, DP, KW>), dim3(grid), dim3(256), 0, s, a);
   } else if (pass == kAttnFwd) {
     hipLaunchKernelGGL((attn_fwd_kernel<T, DP, KW>), dim3(grid), dim3(256), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((attn_dq_kernel<T, DP, KW>), dim3(grid), dim3(256), 0, s, a);
+  } else if (pass == kAttnDq) {
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP, KW, false>), dim3(grid), dim3(256), 0, s, a);
+  } else if constexpr (sizeof(T) == 2) {
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP, KW, true>), dim3(grid), dim3(256), 0, s, a);
   }
 }
 

@@ -122,7 +122,7 @@ def _visible(B, L, S, mask, causal, device):
   return seen
 
 
-def _exact(q, k, v, g, mask, causal, scale):
+def _exact(q, k, v, g, mask, causal, scale, few=False):
   """Outputs, gradients and the bound of each in float64.
 
   With u the half step of the element type (0 for float32 inside the products) and e = 2^-24:
@@ -132,7 +132,8 @@ def _exact(q, k, v, g, mask, causal, scale):
   same with out and by (error of the stored out) |do|; ds = p (dp - delta) by r (+ u) of itself, and so on.  Sums of n
   terms in float32 add e n times the sum of magnitudes.  The hardware's exp2 gives 0 where the result is below the smallest
   normal number, so a probability (of the row's largest, or of the row's sum) is off by another f = 2^-126 at most: f (|dp| +
-  |delta|) in ds and f |do| in each term of dv, f |v| in each of out."""
+  |delta|) in ds and f |do| in each term of dv, f |v| in each of out.
+  few: delta is sum p dp, off by r + e (S + 4) of its terms and by theirs, and the rounding of ds by u of ds itself."""
   import torch
   dtype = q.dtype
   u = 0.0 if dtype is torch.float32 else _half_step(dtype)
@@ -166,7 +167,11 @@ def _exact(q, k, v, g, mask, causal, scale):
   e_out = (r + u) * A + f @ V.abs() + uo * out.abs()
   e_dp = e * (D + 3) * (GO.abs() @ V.abs().transpose(-1, -2).contiguous())
   e_delta = e * (D + 3) * (GO.abs() * out.abs()).sum(-1, keepdim=True) + (GO.abs() * e_out).sum(-1, keepdim=True)
-  e_ds = p * ((r + u + 4 * e) * (dp.abs() + delta.abs()) + e_dp + e_delta) + f * (dp.abs() + delta.abs())
+  e_round = u * (dp.abs() + delta.abs())
+  if few:
+    e_delta = (p * (e_dp + (r + e * (S + 4)) * dp.abs()) + f * dp.abs()).sum(-1, keepdim=True)
+    e_round = u * (dp - delta).abs()
+  e_ds = p * ((r + 4 * e) * (dp.abs() + delta.abs()) + e_round + e_dp + e_delta) + f * (dp.abs() + delta.abs())
   if dtype is torch.float16:                      # below the type's normal range, after the scaling by powers of two
     e_ds = e_ds + 2.0 ** -34 * ds.abs().amax(-1, keepdim=True) if S else e_ds
     e_ds = e_ds + 2.0 ** -34 * ds.abs().amax(-2, keepdim=True) if L else e_ds
@@ -274,6 +279,31 @@ def test_attention_scales_and_large_scores(name):
   """A scale of the caller's, and scores of several hundred: probabilities that are 1 for one key and 0 for the others."""
   _check(8, name, 2, 40, 70, 2, 2, 64, 'ragged', False, scale=0.03)
   _check(9, name, 2, 40, 70, 2, 2, 64, None, False, scale=1.0, spread=3.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', TYPES)
+@pytest.mark.parametrize('shape', [
+    (2, 9, 1, 2, 1, 24, None, False),
+    (3, 40, 2, 4, 2, 32, None, False),
+    (2, 70, 5, 2, 2, 64, None, False),
+    (2, 50, 50, 4, 1, 128, None, True),
+    (3, 40, 640, 2, 2, 40, 'first three', False),    # the queries' keys would be split
+    (16, 130, 60, 16, 16, 64, 'ragged', False),      # 128 columns a workgroup
+    (16, 130, 130, 16, 16, 36, None, True),
+    (17, 129, 256, 8, 8, 128, 'scattered', False),
+], ids=lambda s: 'x'.join(str(v) for v in s))
+def test_gradients_over_few_keys(name, shape):
+  """Values with a common part, which dp - delta cancels: the gradients have the roundings of ds and of the result alone
+  (delta from the stored output would add its rounding of the common part)."""
+  import torch
+  B, L, S, H, G, D, mask, causal = shape
+  (q, k, v), go, m = _make(31, getattr(torch, name), B, L, S, H, G, D, None if mask == 'first three' else mask)
+  if mask == 'first three':
+    m = (torch.arange(S) >= 3).expand(B, S).cuda()
+  v = (v.float() + 8.0).to(v.dtype)
+  want, bound = _exact(q, k, v, go, m, causal, D ** -0.5, few=name != 'float32')
+  _compare(_run([q, k, v], go, m, causal), want, bound)
 
 
 @pytest.mark.gpu
