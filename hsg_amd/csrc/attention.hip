@@ -200,7 +200,7 @@ int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
   a.delta = w.delta; a.part = w.part; a.part2 = w.part2;
   if (a.C > 0) {
     const AttnPlan p = attn_plan(*args, kAttnDq);
-    if (args->dtype != 0) a.have_delta = a.pad || a.S <= kAttnExactKeys ? 1 : a.causal ? 2 : 0;   // queries of few keys
+    if (args->dtype != 0) a.have_delta = a.pad || a.S <= exact_keys(padded_width(a.D)) ? 1 : a.causal ? 2 : 0;   // queries of few keys
     if (a.have_delta) {
       a.splits = 1;
       if (int rc = attn_go(args->dtype, kAttnDelta, a, p.shape, s)) return rc;

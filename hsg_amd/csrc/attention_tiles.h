@@ -723,10 +723,12 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_jo
 //
 // delta = do . o carries the rounding of a 16-bit o: as much as one of do . v, while what is left of dp - delta over few
 // keys is no more (relative error of dq against 64 bits, where rounding the exact dq gives 1: 2.3 for 2 keys, 1.55 for 16,
-// 1.46 for 128, more where values have a common part).  Queries that see at most kAttnExactKeys keys therefore get delta =
-// sum p dp, summed in float32 by a launch of its own, whose two products they can afford (1.42 for every length; 96 heads
-// x 197 x 197, width 64, bfloat16: 11 us beside 12 + 14 + 15 for forward, dq, dk and dv).
-constexpr int kAttnExactKeys = 256;
+// 1.46 for 128, more where values have a common part).  It enters dq times the mean key, which narrow heads follow closely
+// (width 24, 451 keys: 1.49).  Queries that see at most exact_keys() keys therefore get delta = sum p dp, summed in float32
+// by a launch of its own, whose two products they can afford (1.43 then; 96 heads x 197 x 197, width 64, bfloat16: 11 us
+// beside 12 + 14 + 15 for forward, dq, dk and dv; 40 heads x 451 x 451, width 24, float16: 9 us
+// beside 12 + 12 + 13).
+constexpr int exact_keys(int padded_width) { return padded_width == 32 ? 4096 : 256; }
 
 template <typename T, int DP, int KW, bool SUM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))
@@ -747,7 +749,7 @@ void attn_dq_kernel(const AttnArgs a) {
   key_range(a, at.sp, TR, c0, Sh::COLS, lo, hi, first_limit);
   int last, last_h;                                                   // 2: whose last query sees few keys, whatever the split
   col_of(a, min(c0 + Sh::COLS, a.C) - 1, last, last_h);
-  const bool there = a.have_delta == 1 || (a.have_delta == 2 && last + a.S - a.L < kAttnExactKeys);
+  const bool there = a.have_delta == 1 || (a.have_delta == 2 && last + a.S - a.L < exact_keys(DP));
   if (SUM && !there) return;
   auto tile = [&](int buf, int which) { return reinterpret_cast<T *>(lds + (2 * buf + which) * Sh::TILE); };
   clear_tiles<2 * Sh::NBUF * Sh::TILE>(lds, a.DL < DP);
@@ -770,7 +772,7 @@ void attn_dq_kernel(const AttnArgs a) {
   const int lim = a.causal ? i + a.S - a.L : a.S;
   const float lse = mine ? a.lse[col_at] : __builtin_inff();
   if (pad && lo < hi) hi = visible_end(pad, lo, hi, red);
-  const bool exact = SUM && hi - lo <= kAttnExactKeys;
+  const bool exact = SUM && hi - lo <= exact_keys(DP);
   float delta = 0.0f;
   if (!SUM && there) {
     if (mine) delta = a.delta[col_at];

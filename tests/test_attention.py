@@ -292,6 +292,7 @@ def test_attention_scales_and_large_scores(name):
     (16, 130, 60, 16, 16, 64, 'ragged', False),      # 128 columns a workgroup
     (16, 130, 130, 16, 16, 36, None, True),
     (17, 129, 256, 8, 8, 128, 'scattered', False),
+    (2, 60, 700, 2, 1, 24, 'ragged', False),         # narrow heads: more keys are few
 ], ids=lambda s: 'x'.join(str(v) for v in s))
 def test_gradients_over_few_keys(name, shape):
   """Values with a common part, which dp - delta cancels: the gradients have the roundings of ds and of the result alone
