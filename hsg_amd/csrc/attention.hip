@@ -82,6 +82,13 @@ static AttnSpace attn_space(const hsgk_attention_args &a, bool backward, void *b
   return w;
 }
 
+// workgroups of a pass
+static int64_t attn_groups(const hsgk_attention_args &a, AttnPass pass) {
+  const AttnPlan p = attn_plan(a, pass);
+  const int64_t columns = pass == kAttnDkv ? a.S : (int64_t)a.L * (a.H / a.G), per = p.shape == kAttnWide ? 128 : 32;
+  return (int64_t)a.B * a.G * ((columns + per - 1) / per) * p.splits;
+}
+
 static int attn_check(const hsgk_attention_args *p, bool backward) {
   HSGK_REQUIRE(p, "null argument");
   const hsgk_attention_args &a = *p;
@@ -89,12 +96,14 @@ static int attn_check(const hsgk_attention_args *p, bool backward) {
   HSGK_REQUIRE(a.B >= 0 && a.L >= 0 && a.S >= 0, "negative size");
   HSGK_REQUIRE(a.H >= 1 && a.G >= 1 && a.H % a.G == 0, "the query heads are a multiple of the key heads");
   HSGK_REQUIRE(a.D >= 1 && a.D <= HSGK_ATTENTION_MAX_WIDTH, "head width outside 1 .. 128");
-  HSGK_REQUIRE(isfinite(a.scale) && a.scale > 0.0f, "the scale is positive and finite");
+  HSGK_REQUIRE(a.scale > 0.0f && isfinite(a.scale * 1.4426950408889634f), "the scale is positive and finite");
   const int64_t C = (int64_t)a.L * (a.H / a.G), most = (int64_t)1 << 30;
   HSGK_REQUIRE(C <= most && a.S <= most, "more than 2^30 rows a head");
   const int64_t rows = (C > a.S ? C : a.S) + 128;
   HSGK_REQUIRE((int64_t)a.B * a.G <= most && (int64_t)a.B * a.G * rows <= ((int64_t)1 << 38) / padded_width(a.D),
                "more rows than one launch covers");
+  const int64_t grid = ((int64_t)1 << 24) - 1;                // of 256 threads each
+  HSGK_REQUIRE(attn_groups(a, kAttnFwd) <= grid && (!backward || attn_groups(a, kAttnDkv) <= grid), "more rows than one launch covers");
   const bool some = (int64_t)a.B * a.L > 0, keys = (int64_t)a.B * a.S > 0;
   HSGK_REQUIRE(!some || (a.q && a.out), "null argument");
   HSGK_REQUIRE(!keys || (a.k && a.v), "null argument");

@@ -447,10 +447,22 @@ template <typename T, bool NT> static void distill_launch(const DistillArgs &a, 
   }
 }
 
+constexpr int64_t kDistillRows = (int64_t)1 << 23;         // of a launch, which takes fewer than 2^32 threads
+
 template <typename T> static int distill_run(const DistillArgs &a, bool backward, hipStream_t s) {
-  if (a.n * a.V * (int64_t)sizeof(T) > kDistillCache) distill_launch<T, true>(a, backward, s);
-  else distill_launch<T, false>(a, backward, s);
-  HSGK_LAUNCH_CHECK();
+  const bool nt = a.n * a.V * (int64_t)sizeof(T) > kDistillCache;
+  for (int64_t r = 0; r < a.n; r += kDistillRows) {
+    DistillArgs b = a;
+    b.n = a.n - r < kDistillRows ? a.n - r : kDistillRows;
+    b.z = static_cast<const T *>(a.z) + r * a.stride;
+    if (a.k) { b.t = a.t + r * a.k; b.idx = a.idx + r * a.k; }
+    if (a.stats) b.stats = a.stats + 2 * r;
+    if (backward) { b.g = a.g + r; b.dz = static_cast<T *>(a.dz) + r * a.V; }
+    else b.loss = a.loss + r;
+    if (nt) distill_launch<T, true>(b, backward, s);
+    else distill_launch<T, false>(b, backward, s);
+    HSGK_LAUNCH_CHECK();
+  }
   return 0;
 }
 
@@ -460,7 +472,8 @@ static int distill_check(const void *logits, int dtype, int64_t n, int64_t V, in
   HSGK_REQUIRE(n >= 0 && n < ((int64_t)1 << 31), "rows outside 0 .. 2^31 - 1");
   HSGK_REQUIRE(V >= 1 && V < ((int64_t)1 << 31), "classes outside 1 .. 2^31 - 1");
   HSGK_REQUIRE(k >= 0 && k <= kDistillMax, "teacher entries outside 0 .. HSGK_DISTILL_MAX_K");
-  HSGK_REQUIRE(isfinite(temperature) && temperature > 0.0f, "the temperature is positive and finite");
+  HSGK_REQUIRE(isfinite(temperature) && temperature > 0.0f && isfinite(1.4426950408889634f / temperature),
+               "the temperature is positive and finite, and so is its inverse");
   HSGK_REQUIRE(n == 0 || (logits && (k == 0 || (teacher && index))), "null argument");
   HSGK_REQUIRE(row_stride >= 0, "negative stride");
   HSGK_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == 0 ? 4 : 2) == 0, "the logits are not aligned to their elements");

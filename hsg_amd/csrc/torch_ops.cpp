@@ -672,6 +672,23 @@ void set_strides(int64_t (&st)[3], const Tensor &t) {
   for (int i = 0; i < 3; ++i) st[i] = t.stride(i);
 }
 
+// gradients under create_graph: differentiating them again raises (they would pass for constants)
+struct OnceFn : public torch::autograd::Function<OnceFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &grad, const Tensor &, const Tensor &, const Tensor &, const Tensor &) {
+    return grad.view_as(grad);
+  }
+  static variable_list backward(AutogradContext *, variable_list) {
+    TORCH_CHECK(false, "hsgk::attention and hsgk::topk_distill are differentiable once");
+  }
+};
+
+variable_list once_differentiable(variable_list grads, const Tensor &a, const Tensor &b, const Tensor &c, const Tensor &d) {
+  if (at::GradMode::is_enabled())
+    for (Tensor &g : grads)
+      if (g.defined()) g = OnceFn::apply(g, a, b, c, d);
+  return grads;
+}
+
 hsgk_attention_args attention_args(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &pad, bool causal,
                                    double scale, const Tensor &out) {
   hsgk_attention_args a{};
@@ -681,6 +698,8 @@ hsgk_attention_args attention_args(const Tensor &q, const Tensor &k, const Tenso
     a.padding = static_cast<const uint8_t *>(pad.data_ptr());
     a.padding_stride = pad.stride(0);
   }
+  for (const Tensor *t : {&q, &k})
+    for (const int64_t n : t->sizes()) TORCH_CHECK(n <= (int64_t)1 << 30, "hsgk::attention: a dimension is longer than 2^30");
   a.dtype = type_code(q);
   a.B = (int32_t)q.size(0); a.L = (int32_t)q.size(1); a.H = (int32_t)q.size(2); a.D = (int32_t)q.size(3);
   a.S = (int32_t)k.size(1); a.G = (int32_t)k.size(2);
@@ -720,7 +739,7 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
     auto sv = ctx->get_saved_variables();
     const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &pad = sv[3], &out = sv[4], &lse = sv[5];
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-    Tensor g = last_contiguous(grads[0]);
+    const Tensor incoming = grads[0], g = last_contiguous(incoming);
     Tensor dq = at::empty(q.sizes(), q.options()), dk, dv;
     hsgk_attention_args a = attention_args(q, k, v, pad, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), out);
     a.lse = lse.data_ptr<float>();
@@ -741,7 +760,7 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
       a.workspace_bytes = wsb;
     }
     check(hsgk_attention_bwd(&a, stream_of(q)), "hsgk_attention_bwd");
-    return {dq, want_k ? dk : Tensor(), want_v ? dv : Tensor(), Tensor(), Tensor(), Tensor()};
+    return once_differentiable({dq, want_k ? dk : Tensor(), want_v ? dv : Tensor(), Tensor(), Tensor(), Tensor()}, q, k, v, incoming);
   }
 };
 
@@ -790,13 +809,13 @@ struct TopkDistillFn : public torch::autograd::Function<TopkDistillFn> {
     auto sv = ctx->get_saved_variables();
     const Tensor &z = sv[0], &t = sv[1], &idx = sv[2], &stats = sv[3];
     c10::hip::HIPGuardMasqueradingAsCUDA guard(z.device());
-    Tensor g = grads[0].to(at::kFloat).contiguous();
+    const Tensor incoming = grads[0], g = incoming.to(at::kFloat).contiguous();
     Tensor dz = at::empty(z.sizes(), z.options());
     check(hsgk_topk_distill_bwd(z.data_ptr(), type_code(z), z.size(0), z.size(1), z.stride(0), t.data_ptr<float>(),
                                 idx.data_ptr<int64_t>(), (int)t.size(1), (float)ctx->saved_data["temperature"].toDouble(),
                                 stats.data_ptr<float>(), g.data_ptr<float>(), dz.data_ptr(), stream_of(z)),
           "hsgk_topk_distill_bwd");
-    return {dz, Tensor(), Tensor(), Tensor()};
+    return once_differentiable({dz, Tensor(), Tensor(), Tensor()}, z, z, z, incoming);
   }
 };
 

@@ -194,7 +194,28 @@ def _last_contiguous(t):
   return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+class _Once(torch.autograd.Function):
+  """The first argument; differentiating it raises."""
+
+  @staticmethod
+  def forward(ctx, grad, *inputs):
+    return grad.view_as(grad)
+
+  @staticmethod
+  def backward(ctx, g):
+    raise RuntimeError('attention and topk_distill are differentiable once')
+
+
+def _once_differentiable(grads, *inputs):
+  """Gradients under create_graph: differentiating them again raises (they would pass for constants)."""
+  if not torch.is_grad_enabled():
+    return grads
+  return tuple(g if g is None else _Once.apply(g, *inputs) for g in grads)
+
+
 def _attention_args(q, k, v, padding, causal, scale, out):
+  if max(q.shape + k.shape) > 1 << 30:
+    raise _lib.HsgkError('attention: a dimension is longer than 2^30')
   a = _lib.AttentionArgs()
   a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
   a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
@@ -251,7 +272,8 @@ class Attention(torch.autograd.Function):
         dv = torch.empty(v.shape, dtype=v.dtype, device=dev)
         a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
       _attention_call(_lib.lib().hsgk_attention_bwd, a, 1, dev)
-    return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None)
+    grads = (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None)
+    return _once_differentiable(grads, q, k, v, gout)
 
 
 def attention(q, k, v, padding, causal, scale):
@@ -292,7 +314,7 @@ class TopkDistill(torch.autograd.Function):
       _lib.check(_lib.lib().hsgk_topk_distill_bwd(
           z.data_ptr(), _TYPE_CODES[z.dtype], n, V, z.stride(0), teacher.data_ptr(), index.data_ptr(), teacher.shape[1],
           ctypes.c_float(ctx.temperature), stats.data_ptr(), g.data_ptr(), dz.data_ptr(), _lib.stream_ptr()))
-    return dz, None, None, None
+    return _once_differentiable((dz, None, None, None), z, gloss)
 
 
 def topk_distill(z, teacher, index, temperature):

@@ -86,6 +86,19 @@ def test_c_entry_refuses_bad_arguments():
   assert L.hsgk_attention_fwd(ctypes.byref(a), None) == 0
 
 
+def test_c_entry_refuses_more_than_a_launch_covers():
+  from hsg_amd import _lib
+  L = _lib.lib()
+  buf = ctypes.create_string_buffer(1 << 16)
+  base = (ctypes.addressof(buf) + 255) // 256 * 256
+  for B, Lq, scale in ((1 << 24, 1, 0.5), (1 << 22, 129, 0.5), (1, 1, 3e38)):
+    a = _lib.AttentionArgs()
+    a.q = a.k = a.v = a.out = base
+    a.B, a.L, a.S, a.H, a.G, a.D, a.scale = B, Lq, 3, 4, 4, 8, scale
+    assert L.hsgk_attention_fwd(ctypes.byref(a), None) == -1
+    assert (b'scale' if scale > 1 else b'launch') in L.hsgk_last_error()
+
+
 def test_module_refuses_what_the_kernels_do_not_offer():
   import torch
   from hsg_amd.models.embeddings import transformer_clusters as tc
@@ -263,6 +276,8 @@ SHAPES = [                            # B, L, S, H, G, D, mask, causal
     (17, 129, 150, 8, 8, 128, 'scattered', False),
     (8, 512, 300, 8, 8, 64, None, False),        # ... and the streamed rows in two parts
     (8, 300, 512, 16, 8, 48, None, True),
+    (2, 400, 300, 2, 1, 64, None, True),         # the first 100 queries see no key, many see few
+    (1, 900, 900, 2, 1, 36, None, True),         # few heads: both sides in parts
 ]
 
 
@@ -417,6 +432,34 @@ def test_only_wanted_gradients():
     got = torch.autograd.grad(out, [leaves[i] for i in pick], go)
     for i, g in zip(pick, got):
       assert torch.equal(g, want[('dq', 'dk', 'dv')[i]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('binding', ['torch', 'ctypes'])
+def test_gradients_cannot_be_differentiated(binding, monkeypatch):
+  """create_graph works, and a gradient of the gradient raises instead of counting as zero."""
+  import torch
+  if binding == 'ctypes':
+    monkeypatch.setenv('HSGK_BINDING', 'ctypes')
+  from hsg_amd.models.embeddings.transformer_clusters import attention
+  t, go, _ = _make(5, torch.float32, 2, 9, 11, 2, 2, 16)
+  leaves = [x.requires_grad_(True) for x in t]
+  want = torch.autograd.grad(attention(*leaves), leaves, go)
+  got = torch.autograd.grad(attention(*leaves), leaves, go, create_graph=True)
+  for a, b in zip(got, want):
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+      torch.autograd.grad(a.sum(), leaves, allow_unused=True, retain_graph=True)
+
+
+@pytest.mark.gpu
+def test_a_dimension_that_32_bits_do_not_hold_is_refused():
+  import torch
+  from hsg_amd.models.embeddings.transformer_clusters import attention
+  q = torch.zeros((1, 2, 1, 4), device='cuda')
+  k = torch.zeros((1, 1, 1, 4), device='cuda').expand(1, (1 << 32) + 5, 1, 4)
+  with pytest.raises(RuntimeError):
+    attention(q, k, k)
 
 
 @pytest.mark.gpu
@@ -597,4 +640,5 @@ def test_module_equals_torchs(batch_first):
     a, w = ours(*io, key_padding_mask=mask)
     b, _ = ref.double()(*[x.double() for x in io], key_padding_mask=mask)
     assert w is None and a.shape == b.shape
+    a, b = a.detach(), b.detach()
     assert float((a.double() - b).norm()) <= 2.0 ** -24 * 400 * float(b.norm())   # three products of 24 .. 48 terms and the rows

@@ -63,6 +63,7 @@ def test_c_entry_refuses_bad_arguments():
     args[i] = None
     assert L.hsgk_topk_distill_bwd(*args, None) == -1, i
   assert L.hsgk_topk_distill_fwd(None, 0, 0, 8, 8, None, None, 4, 1.0, None, None, None) == 0     # no rows
+  assert L.hsgk_topk_distill_fwd(*good[:8], 1e-39, *good[9:], None) == -1                         # 1 / T is infinite
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -262,6 +263,28 @@ def test_gradient_against_differences():
   slope = float(((up - down) * g.double()).sum()) / (2 * h)
   inner = float((dz.double() * d.double()).sum())
   assert abs(slope - inner) <= 1e-5 * (1 + float(dz.double().norm()) * float(d.double().norm()))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_takes():
+  import torch
+  _check(*_make(23, torch.float16, (1 << 23) + 3, 6, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('binding', ['torch', 'ctypes'])
+def test_gradient_cannot_be_differentiated(binding, monkeypatch):
+  import torch
+  from hsg_amd.utils.segsort.loss import topk_distillation_loss
+  if binding == 'ctypes':
+    monkeypatch.setenv('HSGK_BINDING', 'ctypes')
+  z, t, idx, _ = _make(3, torch.float32, 5, 40, 3)
+  z.requires_grad_(True)
+  (want,) = torch.autograd.grad(topk_distillation_loss(z, t, idx), z)
+  (got,) = torch.autograd.grad(topk_distillation_loss(z, t, idx), z, create_graph=True)
+  assert torch.equal(got, want)
+  with pytest.raises(RuntimeError, match='differentiable once'):
+    torch.autograd.grad(got.sum(), z)
 
 
 @pytest.mark.gpu
