@@ -57,7 +57,7 @@ template <> struct Elem<_Float16> { static constexpr int KS = 16, MMA = 1; };
 
 // The order of READS LDS reads and MMAS matrix instructions of the code before this line: AHEAD reads first, then in turn,
 // so that an operand is on its way while the matrix unit works on earlier ones (the compiler alone keeps two in flight; dk
-// and dv at width 128, one wave a SIMD: 909 us without, 857 with it; other kernels 0 - 3 %).
+// and dv at width 128, one wave a SIMD: 830 us without, 777 with it; the other kernels gain nothing and lose nothing).
 template <int READS, int MMAS, int AHEAD> __device__ __forceinline__ void read_ahead() {
   constexpr int A = AHEAD < READS ? AHEAD : READS, PER = MMAS / READS;
   __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
@@ -411,7 +411,7 @@ template <int BYTES> __device__ __forceinline__ void clear_tiles(unsigned char *
 // multiple of 8 a head still stays on its XCDs).  Parts of split rows are
 // counted from the end that every block sees, so the first parts are whole, and neighbours in the order differ little: within
 // an XCD workgroups are placed in order, and one that has to wait holds up the rest (dk and dv of 16 heads on 4, 8192 x 8192,
-// width 128: 1318 us with the two parts of a block next to each other, 857 this way).
+// width 128: 1.54 times as long with the two parts of a block next to each other).
 struct Place {
   int sp, cb, bg;
 };
@@ -521,7 +521,11 @@ template <typename T, int DP, int TR> struct KeyRows {
   __device__ __forceinline__ uint32_t bits_of(int r0, int h) const { return (uint32_t)(word(r0 >> 6) >> ((r0 & 63) + 4 * h)); }
 };
 // ---------------------------------------------------------------------------------------------------------------------
-// forward: columns = queries, keys and values stream
+// forward: columns = queries, keys and values stream.  Long sequences are bound by the matrix and the vector unit in turn (of
+// the two waves of a SIMD one rarely multiplies while the other takes its exponentials): 24 heads x 2305 x 2305, width 64,
+// bfloat16, 58 us, 560 TFLOP/s; 16 heads x 8192 x 8192 causal, width 128, 310 us, 890 TFLOP/s (a large matrix product 1130);
+// float32 is bound by its matrix instructions.  Few queries are bound by the keys and values: one token of 16 heads on 4, 2 x
+// 32768 keys, width 128, 26 + 4 us, 5.1 TB/s (a large copy 5.2).
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))
 void attn_fwd_kernel(const AttnArgs a) {
@@ -719,15 +723,15 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_jo
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dq, or with SUM delta alone: columns = queries, keys and values stream
+// dq, or with SUM delta alone: columns = queries, keys and values stream; three products, bound like the forward pass (the
+// two shapes there: 70 us, 700 TFLOP/s, and 405 us, 1020 TFLOP/s)
 //
 // delta = do . o carries the rounding of a 16-bit o: as much as one of do . v, while what is left of dp - delta over few
 // keys is no more (relative error of dq against 64 bits, where rounding the exact dq gives 1: 2.3 for 2 keys, 1.55 for 16,
 // 1.46 for 128, more where values have a common part).  It enters dq times the mean key, which narrow heads follow closely
 // (width 24, 451 keys: 1.49).  Queries that see at most exact_keys() keys therefore get delta = sum p dp, summed in float32
 // by a launch of its own, whose two products they can afford (1.43 then; 96 heads x 197 x 197, width 64, bfloat16: 11 us
-// beside 12 + 14 + 15 for forward, dq, dk and dv; 40 heads x 451 x 451, width 24, float16: 9 us
-// beside 12 + 12 + 13).
+// beside 12 + 14 + 15 for forward, dq, dk and dv; 40 heads x 451 x 451, width 24, float16: 9 us beside 12 + 12 + 13).
 constexpr int exact_keys(int padded_width) { return padded_width == 32 ? 4096 : 256; }
 
 template <typename T, int DP, int KW, bool SUM>
@@ -879,8 +883,10 @@ void attn_dq_kernel(const AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// dk and dv: columns = keys, the queries that use this key head and their output gradients stream; the heads of a
-// group are rows of the same stream, so shared heads are summed here, in a fixed order and without atomics
+// dk and dv: columns = keys, the queries that use this key head and their output gradients stream; the heads of a group are
+// rows of the same stream, so shared heads are summed here, in a fixed order and without atomics.  Four products; the two
+// shapes above: 85 us, 770 TFLOP/s, and 750 us, 730 TFLOP/s (at width 128 the sums of dk and dv leave registers for one wave
+// a SIMD, which waits for its own exponentials).
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WB)))
 void attn_dkv_kernel(const AttnArgs a) {

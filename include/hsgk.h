@@ -507,7 +507,10 @@ HSGK_API int hsgk_synth_mixture(uint64_t noise_key, uint64_t seed, const float *
  * the last dimension is contiguous; out, dq, dk and dv are contiguous and 16-byte aligned.  1 <= D <= 128, scale > 0.
  * lse float32 [B,G,L,H/G] (forward: nullable; backward: what the forward wrote): log2 of the sum of 2^(score log2 e).
  * backward: reads out and lse of the forward, recomputes the probabilities, writes dq and (both or neither) dk, dv; no
- * atomics, the order of every sum is fixed.  The workspace belongs to one call at a time.                            */
+ * atomics, the order of every sum is fixed.  The backward sums delta = sum_j p_j (dout_i . v_j) in float32 where a query
+ * sees few keys, and takes dout_i . out_i elsewhere.
+ * Workspace: 16-byte aligned, of one call at a time; its size depends on the sizes and on whether the rows of q, k, v (and
+ * dout) can be read in aligned 16-byte pieces, so ask with their pointers and strides set (rows that cannot are copied).  */
 #define HSGK_ATTENTION_MAX_WIDTH 128
 typedef struct hsgk_attention_args {
   const void *q, *k, *v;
