@@ -325,6 +325,11 @@ template <typename T, int DB> struct ColumnScale {
 template <typename T> constexpr float prob_shift() {         // log2 of the factor the probabilities carry into float16
   return sizeof(T) == 2 && !__is_same(T, __bf16) ? 15.0f : 0.0f;
 }
+// the forward pass scales what it has summed so far only when a maximum has grown by 2^kAttnLazy, so that probabilities may
+// reach that meanwhile (a maximum of many columns grows in almost every tile otherwise: 16 heads x 8192 x 8192 causal, width
+// 128, bfloat16, 320 us; 301 this way)
+constexpr float kAttnLazy = 8.0f;
+template <typename T> constexpr float fwd_shift() { return prob_shift<T>() == 0.0f ? 0.0f : prob_shift<T>() - kAttnLazy; }
 
 // A workgroup of four waves with 32 columns each (KW = 1), or with the same 32 columns, each wave on a quarter of every
 // tile's rows, their results joined at the end (KW = 4: few columns).
@@ -523,7 +528,7 @@ template <typename T, int DP, int TR> struct KeyRows {
 // ---------------------------------------------------------------------------------------------------------------------
 // forward: columns = queries, keys and values stream.  Long sequences are bound by the matrix and the vector unit in turn (of
 // the two waves of a SIMD one rarely multiplies while the other takes its exponentials): 24 heads x 2305 x 2305, width 64,
-// bfloat16, 58 us, 560 TFLOP/s; 16 heads x 8192 x 8192 causal, width 128, 310 us, 890 TFLOP/s (a large matrix product 1130);
+// bfloat16, 57 us, 570 TFLOP/s; 16 heads x 8192 x 8192 causal, width 128, 295 us, 930 TFLOP/s (a large matrix product 1130);
 // float32 is bound by its matrix instructions.  Few queries are bound by the keys and values: one token of 16 heads on 4, 2 x
 // 32768 keys, width 128, 26 + 4 us, 5.1 TB/s (a large copy 5.2).
 template <typename T, int DP, int KW>
@@ -600,7 +605,7 @@ void attn_fwd_kernel(const AttnArgs a) {
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[x][r]);
     top = both_max(top);
     const float mn = fmaxf(m, top);
-    if (__any(mn > m)) {                                              // (a column whose maximum stays: factor 1)
+    if (__any((mn - m) * a.c2 > kAttnLazy)) {                         // (a column whose maximum stays: factor 1)
       const float f = mn > m ? exp2f((m - mn) * a.c2) : 1.0f;
       l *= f;
 #pragma unroll
@@ -609,7 +614,7 @@ void attn_fwd_kernel(const AttnArgs a) {
         for (int r = 0; r < 16; ++r) acc[db][r] *= f;
       m = mn;
     }
-    const float base = m == -__builtin_inff() ? 0.0f : prob_shift<T>() - m * a.c2;
+    const float base = m == -__builtin_inff() ? 0.0f : fwd_shift<T>() - m * a.c2;
 #pragma unroll
     for (int x = 0; x < X; ++x)
 #pragma unroll
@@ -637,7 +642,7 @@ void attn_fwd_kernel(const AttnArgs a) {
   stream<TR, Sh::NBUF, Sh::UNROLL>(lo, hi, issue, [&](int buf) { st.land(pad, tile(buf, 0), tile(buf, 1)); }, compute);
 
   l = both_sum(l);
-  const float mt = l == 0.0f ? -__builtin_inff() : m * a.c2 - prob_shift<T>();       // log2 of the factor taken out of l and acc
+  const float mt = l == 0.0f ? -__builtin_inff() : m * a.c2 - fwd_shift<T>();      // log2 of the factor taken out of l and acc
   auto out_row = [&](int ci, int ch) { return static_cast<T *>(a.out) + (((int64_t)b * a.L + ci) * a.H + gh * a.HG + ch) * a.D; };
   const int64_t first = (int64_t)at.bg * a.C, part = (int64_t)at.sp * a.B * a.G * a.C;
   if constexpr (KW > 1) {
