@@ -124,11 +124,55 @@ static int attn_check(const hsgk_attention_args *p, bool backward) {
   return 0;
 }
 
-template <typename T> static int attn_pack(const void *from, const int64_t *st, int64_t B, int n, int heads, int D, int DL, void *to, hipStream_t s) {
-  const int64_t rows = B * n * heads, blocks = (rows * DL + 255) / 256;
+// Rows whose 16-byte pieces are not aligned, copied into aligned ones, zeros past their end: [B, n, heads, pieces].  A thread
+// copies a piece in words of G bytes, 2^lg threads a row (10 x 4158 x 6 rows of 36 bfloat16: 9.2 us, 4.1 TB/s; 30 element by
+// element).
+template <int G> struct Word;
+template <> struct Word<2> { using T = uint16_t; };
+template <> struct Word<4> { using T = uint32_t; };
+template <> struct Word<8> { using T = uint2; };
+
+template <int G>
+__global__ __launch_bounds__(256) void attn_pack_kernel(const char *from, int64_t sb, int64_t sl, int64_t sh, int64_t rows, int n, int heads,
+                                                        int bytes, int pieces, int lg, uint4 *to) {
+  using W = typename Word<G>::T;
+  const int p = (int)threadIdx.x & ((1 << lg) - 1), per = 256 >> lg;
+  if (p >= pieces) return;
+  for (int64_t row = (int64_t)blockIdx.x * per + ((int)threadIdx.x >> lg); row < rows; row += (int64_t)gridDim.x * per) {
+    int64_t b, i;
+    int head;
+    if (rows <= 0x7fffffff) {                              // (a division of 64 bits takes as long as the copy)
+      const unsigned j = (unsigned)row / (unsigned)heads, c = j / (unsigned)n;
+      head = (int)((unsigned)row - j * heads);
+      b = c; i = j - c * n;
+    } else {
+      const int64_t j = row / heads;
+      head = (int)(row - j * heads);
+      b = j / n; i = j - b * n;
+    }
+    const char *src = from + b * sb + i * sl + head * sh + 16 * p;
+    W x[16 / G];
+#pragma unroll
+    for (int c = 0; c < 16 / G; ++c) x[c] = 16 * p + c * G < bytes ? *reinterpret_cast<const W *>(src + c * G) : W{};
+    uint4 y;
+    __builtin_memcpy(&y, x, 16);
+    to[row * pieces + p] = y;
+  }
+}
+
+static int attn_pack(const void *from, const int64_t *st, int size, int64_t B, int n, int heads, int D, int DL, void *to, hipStream_t s) {
+  const int64_t rows = B * n * heads;
   if (rows == 0) return 0;
-  hipLaunchKernelGGL(attn_pack_kernel<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, static_cast<const T *>(from),
-                     st[0], st[1], st[2], rows, n, heads, D, DL, static_cast<T *>(to));
+  const int bytes = D * size, count = DL * size / 16;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(from) | (uintptr_t)(st[0] * size) | (uintptr_t)(st[1] * size) | (uintptr_t)(st[2] * size) |
+                        (uintptr_t)bytes;
+  int lg = 0;
+  while ((1 << lg) < count) ++lg;
+  const int64_t blocks = (rows + (256 >> lg) - 1) / (256 >> lg);
+  const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384)), block(256);
+  const auto kernel = all % 8 == 0 ? attn_pack_kernel<8> : all % 4 == 0 ? attn_pack_kernel<4> : attn_pack_kernel<2>;
+  hipLaunchKernelGGL(kernel, grid, block, 0, s, static_cast<const char *>(from), st[0] * size, st[1] * size, st[2] * size, rows, n, heads,
+                     bytes, count, lg, static_cast<uint4 *>(to));
   HSGK_LAUNCH_CHECK();
   return 0;
 }
@@ -151,8 +195,7 @@ static int attn_args(const hsgk_attention_args &p, const AttnSpace &w, bool back
     }
     const bool query = i == 0 || i == 3;
     const int n = query ? p.L : p.S, heads = query ? p.H : p.G;
-    const int rc = size == 4 ? attn_pack<float>(from[i], st[i], p.B, n, heads, p.D, a.DL, w.packed[i], s)
-                             : attn_pack<_Float16>(from[i], st[i], p.B, n, heads, p.D, a.DL, w.packed[i], s);   // (bits only)
+    const int rc = attn_pack(from[i], st[i], size, p.B, n, heads, p.D, a.DL, w.packed[i], s);
     if (rc) return rc;
     *to[i] = w.packed[i];
     ts[i][0] = (int64_t)n * heads * a.DL; ts[i][1] = (int64_t)heads * a.DL; ts[i][2] = a.DL;

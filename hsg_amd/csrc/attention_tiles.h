@@ -1084,18 +1084,6 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(const float *part, int sp
   }
 }
 
-// rows whose 16-byte pieces are not aligned, copied into aligned ones of DL elements (zeros past D): [B, n, heads, DL]
-template <typename T>
-__global__ __launch_bounds__(256) void attn_pack_kernel(const T *from, int64_t sb, int64_t sl, int64_t sh, int64_t rows, int n,
-                                                        int heads, int D, int DL, T *to) {
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * DL; t += (int64_t)gridDim.x * 256) {
-    const int64_t row = t / DL;
-    const int d = (int)(t - row * DL), hd = (int)(row % heads);
-    const int64_t i = row / heads, b = i / n;
-    to[t] = d < D ? from[b * sb + (i - b * n) * sl + hd * sh + d] : (T)0.0f;
-  }
-}
-
 // ---- launches ---------------------------------------------------------------------------------------------------------
 enum AttnPass { kAttnFwd, kAttnDelta, kAttnDq, kAttnDkv };
 // columns of a workgroup: 32 that its waves share, or 128
