@@ -14,22 +14,26 @@ struct AttnPlan {
   int splits;          // parts of the streamed rows, joined by a second kernel
 };
 
-// Shared columns where 128 of them would leave CUs without a workgroup (float32, 28 heads x 131 queries x 203 keys, width
-// 36: forward, dq, dk and dv 16 + 17 + 25 us shared, 23 + 31 + 49 with 128; 192 heads x 256 x 256, width 32: 32 + 38 + 43
-// shared, 25 + 35 + 42 with 128).  Split rows where there are fewer workgroups than `room`, what the CUs hold at a time:
-// more only add partial results (one token of 16 heads over 2 x 32768 keys, width 128: 256 workgroups 25 + 4 us, 512
-// 30 + 4).  Causal blocks differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys: 1105 us in one
-// part, 760 + 16 in two).
+// Shared columns where all their workgroups run at once, one, two or three a CU by LDS (forward, dq, dk and dv, us, shared and
+// with 128 columns: float32, 28 heads x 131 x 203, width 36, 126 workgroups 16 + 17 + 25 and 23 + 31 + 49; float16, 36 heads x
+// 510 x 510, width 80, 576 workgroups 49 + 46 + 64 and 16 + 25 + 31), and for few columns anyway, of which 128 would be mostly
+// empty (forward and dq; bfloat16, 1024 heads, width 64: 1 column x 2048 keys 106 and 124 forward, 16 x 512 28 + 27 and 26 +
+// 32, 32 x 512 31 + 29 and 26 + 32; float32, 512 heads, width 48: 64 x 512 79 + 93 and 79 + 111, 96 x 512 117 + 139 and 82 +
+// 117).
+// Split rows where there are fewer workgroups than `room`, what the CUs hold at a time: more only add partial results (one token of
+// 16 heads over 2 x 32768 keys, width 128: 256 workgroups 25 + 4 us, 512 30 + 4; 30 heads x 930 x 930, width 72, float32, 240
+// workgroups 143 us, 480 153 + 9).  Causal blocks differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys:
+// 1105 us in one part, 760 + 16 in two).
 static AttnPlan attn_plan(const hsgk_attention_args &a, AttnPass pass) {
   const bool dkv = pass == kAttnDkv;
   const int64_t heads = (int64_t)a.B * a.G, queries = (int64_t)a.L * (a.H / a.G);
   const int64_t columns = dkv ? a.S : queries, rows = dkv ? queries : a.S;
   const int bytes = padded_width(a.D) * elem_size(a.dtype);                 // of a row in LDS
   AttnPlan p;
-  p.shape = columns <= 32 || heads * ((columns + 127) / 128) < 256 ? kAttnShared : kAttnWide;
-  const int64_t per = p.shape == kAttnWide ? 128 : 32, groups = heads * ((columns + per - 1) / per);
-  const bool alone = (p.shape == kAttnShared && bytes >= 256) || (dkv && bytes >= 256);   // LDS or registers hold one workgroup a CU
-  const int64_t room = alone && !a.causal ? 256 : 512;
+  const int64_t shared = heads * ((columns + 31) / 32), at_once = bytes >= 256 ? 256 : bytes >= 128 ? 512 : 768;
+  p.shape = columns <= (a.dtype == 0 ? 64 : 15) || shared <= at_once ? kAttnShared : kAttnWide;
+  const int64_t groups = p.shape == kAttnWide ? heads * ((columns + 127) / 128) : shared;
+  const int64_t room = (p.shape == kAttnWide || bytes >= 256) && !a.causal ? 256 : 512;
   int64_t s = groups > 0 ? room / groups : 1;
   const int64_t most = rows / 256;
   if (s > most) s = most;

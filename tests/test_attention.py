@@ -278,6 +278,10 @@ SHAPES = [                            # B, L, S, H, G, D, mask, causal
     (8, 300, 512, 16, 8, 48, None, True),
     (2, 400, 300, 2, 1, 64, None, True),         # the first 100 queries see no key, many see few
     (1, 900, 900, 2, 1, 36, None, True),         # few heads: both sides in parts
+    (1, 3, 3000, 2, 1, 64, 'scattered', False),  # more than eight parts
+    (5, 300, 600, 8, 8, 128, 'ragged', False),   # 128 columns a workgroup and parts
+    (2, 512, 640, 16, 8, 100, None, True),
+    (70, 40, 50, 8, 8, 64, 'ragged', False),     # many heads of few columns, shared by float32 alone
 ]
 
 

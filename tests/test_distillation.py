@@ -362,6 +362,6 @@ def test_retrieval_attention_and_distillation_together():
   want_loss = step(a64, b64, True)
   want = torch.autograd.grad(want_loss, (a64, b64))
   # products of at most 40 terms, a softmax each way, kappa 8: 2^-24 * 500 of the norm
-  assert abs(float(loss) - float(want_loss)) <= 3e-5 * abs(float(want_loss))
+  assert abs(float(loss.detach()) - float(want_loss.detach())) <= 3e-5 * abs(float(want_loss.detach()))
   for u, v in zip(got, want):
     assert float((u.double() - v).norm()) <= 3e-5 * float(v.norm())
