@@ -6,8 +6,12 @@
 
 namespace hsgk {
 
-static int padded_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 static int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+// (float32, whose products cost seven times as much, also to 96: 30 heads x 930 x 930, width 72, forward, dq, dk and dv 123 + 169 +
+// 222 us, 150 + 210 + 275 with 128)
+static int padded_width(const hsgk_attention_args &a) {
+  return a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.dtype == 0 && a.D <= 96 ? 96 : 128;
+}
 
 struct AttnPlan {
   AttnShape shape;
@@ -28,7 +32,7 @@ static AttnPlan attn_plan(const hsgk_attention_args &a, AttnPass pass) {
   const bool dkv = pass == kAttnDkv;
   const int64_t heads = (int64_t)a.B * a.G, queries = (int64_t)a.L * (a.H / a.G);
   const int64_t columns = dkv ? a.S : queries, rows = dkv ? queries : a.S;
-  const int bytes = padded_width(a.D) * elem_size(a.dtype);                 // of a row in LDS
+  const int bytes = padded_width(a) * elem_size(a.dtype);                 // of a row in LDS
   AttnPlan p;
   const int64_t shared = heads * ((columns + 31) / 32), at_once = bytes >= 256 ? 256 : bytes >= 128 ? 512 : 768;
   p.shape = columns <= (a.dtype == 0 ? 64 : 15) || shared <= at_once ? kAttnShared : kAttnWide;
@@ -60,7 +64,7 @@ static AttnSpace attn_space(const hsgk_attention_args &a, bool backward, void *b
   Carver c(base);
   AttnSpace w = {};
   const int64_t heads = (int64_t)a.B * a.G, C = (int64_t)a.L * (a.H / a.G);
-  const size_t dp = (size_t)padded_width(a.D);
+  const size_t dp = (size_t)padded_width(a);
   const AttnPlan f = attn_plan(a, backward ? kAttnDq : kAttnFwd);
   if (!backward) {
     if (f.splits > 1) {
@@ -104,7 +108,7 @@ static int attn_check(const hsgk_attention_args *p, bool backward) {
   const int64_t C = (int64_t)a.L * (a.H / a.G), most = (int64_t)1 << 30;
   HSGK_REQUIRE(C <= most && a.S <= most, "more than 2^30 rows a head");
   const int64_t rows = (C > a.S ? C : a.S) + 128;
-  HSGK_REQUIRE((int64_t)a.B * a.G <= most && (int64_t)a.B * a.G * rows <= ((int64_t)1 << 38) / padded_width(a.D),
+  HSGK_REQUIRE((int64_t)a.B * a.G <= most && (int64_t)a.B * a.G * rows <= ((int64_t)1 << 38) / padded_width(a),
                "more rows than one launch covers");
   const int64_t grid = ((int64_t)1 << 24) - 1;                // of 256 threads each
   HSGK_REQUIRE(attn_groups(a, kAttnFwd) <= grid && (!backward || attn_groups(a, kAttnDkv) <= grid), "more rows than one launch covers");
@@ -256,7 +260,7 @@ int hsgk_attention_bwd(const hsgk_attention_args *args, hsgk_stream_t stream) {
   a.delta = w.delta; a.part = w.part; a.part2 = w.part2;
   if (a.C > 0) {
     const AttnPlan p = attn_plan(*args, kAttnDq);
-    if (args->dtype != 0) a.have_delta = a.pad || a.S <= exact_keys(padded_width(a.D)) ? 1 : a.causal ? 2 : 0;   // queries of few keys
+    if (args->dtype != 0) a.have_delta = a.pad || a.S <= exact_keys(padded_width(*args)) ? 1 : a.causal ? 2 : 0;   // queries of few keys
     if (a.have_delta) {
       a.splits = 1;
       if (int rc = attn_go(args->dtype, kAttnDelta, a, p.shape, s)) return rc;

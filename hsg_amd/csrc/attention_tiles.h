@@ -1,5 +1,5 @@
 // attention_tiles.h -- the kernels of attention.hip, templates over the element type (float, bf16 as hsgk_bf16,
-// _Float16) and the padded head width DP (32, 64, 128).
+// _Float16) and the padded head width DP (32, 64, 128; float also 96).
 //
 // Mathematics, per (batch item, key head): rows q_c of the queries that use this key head (column c = query position *
 // shared heads + head inside the group), keys k_j, values v_j,
@@ -339,7 +339,7 @@ template <typename T> constexpr float fwd_shift() { return prob_shift<T>() == 0.
 // same 32 columns: 34 -> 47 and, 24 heads x 2305 x 2305, 60 -> 87.)
 template <typename T, int DP, int KW> struct Shape {
   static constexpr int COLS = 128 / KW;                                            // columns of a workgroup
-  static constexpr int TR = KW == 4 ? 128 : sizeof(T) == 4 && DP == 128 ? 32 : 64; // streamed rows per tile
+  static constexpr int TR = KW == 4 ? 128 : sizeof(T) == 4 && DP >= 96 ? 32 : 64;  // streamed rows per tile
   static constexpr int NS = TR / KW / 32;                                          // 32-row blocks of a wave per tile
   static constexpr int TILE = TR * DP * (int)sizeof(T);                            // bytes of one staged tile
   static constexpr int NBUF = 4 * TILE <= 128 * 1024 ? 2 : 1;
@@ -349,8 +349,8 @@ template <typename T, int DP, int KW> struct Shape {
   static constexpr int AHEAD = sizeof(T) == 4 ? 4 : 8;                                            // see read_ahead
   // waves of a SIMD that the registers have to leave room for (no more than the LDS does)
   static constexpr int W0 = LDS > 80 * 1024 ? 1 : LDS > 52 * 1024 ? 2 : 3;
-  static constexpr int WF = DP == 32 ? W0 : W0 < 2 || (sizeof(T) == 4 && DP == 128) ? 1 : 2;
-  static constexpr int WB = DP == 128 ? 1 : WF;
+  static constexpr int WF = DP == 32 ? W0 : W0 < 2 || (sizeof(T) == 4 && DP >= 96) ? 1 : 2;
+  static constexpr int WB = DP >= 96 ? 1 : WF;
 };
 
 // partial results of the waves, for the join (the caller synchronises before and after)
@@ -716,7 +716,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_jo
   float o = 0.0f;
 #pragma unroll 8
   for (int s = y; s < a.splits; s += Y) o = fmaf(a.part[(s * n + at) * DP + d], wt[s], o);
-  red[y][d] = o;
+  if (y < Y) red[y][d] = o;                                           // (256 is no multiple of 96)
   __syncthreads();
   if (y) return;
   for (int x = 1; x < Y; ++x) o += red[x][d];
@@ -1156,6 +1156,9 @@ template <typename T, int DP, bool DKV> int attn_run(AttnPass pass, const AttnAr
 template <typename T, bool DKV> int attn_type(AttnPass pass, const AttnArgs &a, AttnShape shape, hipStream_t s) {
   if (a.D <= 32) return attn_run<T, 32, DKV>(pass, a, shape, s);
   if (a.D <= 64) return attn_run<T, 64, DKV>(pass, a, shape, s);
+  if constexpr (sizeof(T) == 4) {
+    if (a.D <= 96) return attn_run<T, 96, DKV>(pass, a, shape, s);
+  }
   return attn_run<T, 128, DKV>(pass, a, shape, s);
 }
 

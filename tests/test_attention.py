@@ -282,6 +282,10 @@ SHAPES = [                            # B, L, S, H, G, D, mask, causal
     (5, 300, 600, 8, 8, 128, 'ragged', False),   # 128 columns a workgroup and parts
     (2, 512, 640, 16, 8, 100, None, True),
     (70, 40, 50, 8, 8, 64, 'ragged', False),     # many heads of few columns, shared by float32 alone
+    (12, 129, 150, 8, 8, 80, 'ragged', False),   # float32: padded to 96
+    (2, 300, 330, 12, 4, 96, None, True),
+    (1, 3, 3000, 2, 1, 90, 'scattered', False),
+    (3, 70, 600, 4, 2, 65, 'ragged', False),
 ]
 
 
