@@ -40,6 +40,15 @@ static AttnPlan attn_plan(const hsgk_attention_args &a, AttnPass pass) {
   const int64_t room = (p.shape == kAttnWide || bytes >= 256) && !a.causal ? 256 : 512;
   int64_t s = groups > 0 ? room / groups : 1;
   const int64_t most = rows / 256;
+  if (s < 1) s = 1;
+  if (p.shape == kAttnShared && bytes >= 256 && !a.causal && groups <= room) {
+    // rounds of the CUs over parts: 160 workgroups leave a hundred CUs idle, three times as many take two rounds of a third (one
+    // token of 32 heads on 8, 20 x 8192 keys, width 128, bfloat16: 155 us, 134 + 5; two workgroups a CU fill it as they are)
+    auto time = [&](int64_t parts) { return (double)((groups * parts + room - 1) / room) / (double)parts; };
+    const int64_t first = s;
+    for (int64_t t = first + 1; t <= first + 3; ++t)
+      if (time(t) < 0.9 * time(s)) s = t;
+  }
   if (s > most) s = most;
   if (s > kAttnMaxSplits) s = kAttnMaxSplits;
   p.splits = s > 1 ? (int)s : 1;

@@ -286,6 +286,7 @@ SHAPES = [                            # B, L, S, H, G, D, mask, causal
     (2, 300, 330, 12, 4, 96, None, True),
     (1, 3, 3000, 2, 1, 90, 'scattered', False),
     (3, 70, 600, 4, 2, 65, 'ragged', False),
+    (20, 1, 900, 32, 8, 128, 'ragged', False),   # 160 workgroups: three parts
 ]
 
 
