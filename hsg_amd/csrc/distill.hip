@@ -92,11 +92,10 @@ template <bool NT> __device__ __forceinline__ uint4 load16(const uint4 *p) {
   return NT ? __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4nt *>(p))) : *p;
 }
 
-// exp2 of (x - base) / T.  Logits of 16 bits take one instruction for the argument (base2 = base c2 rounded: 2^-24 of an
-// exponent's size, the same for the whole row); float32 subtracts first.
-template <typename T> __device__ __forceinline__ float power(float x, float base, float base2, float c2) {
-  return __builtin_amdgcn_exp2f(sizeof(T) == 2 ? fmaf(x, c2, -base2) : (x - base) * c2);
-}
+// exp2 of (x - base) / T.  The difference comes first: it is exact for 16-bit logits and small where it matters, while
+// x c2 - base c2 would carry the rounding of base c2, which what all logits of a row have in common makes large (float16, an
+// offset of 1000, T = 0.5: log L off by up to 8e-5) and which the lowest value of bfloat16 takes past float32's range.
+__device__ __forceinline__ float power(float x, float base, float c2) { return __builtin_amdgcn_exp2f((x - base) * c2); }
 
 template <typename T> __device__ __forceinline__ void widen(const uint4 &u, float (&x)[Piece<T>::E]) {
   T y[Piece<T>::E];
@@ -215,7 +214,7 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_fw
     for (int e = 0; e < n; ++e) top = fmaxf(top, x[e]);
     const float base = top == -__builtin_inff() ? 0.0f : top;
     l *= __builtin_amdgcn_exp2f((m - base) * a.c2);
-    for (int e = 0; e < n; ++e) l += power<T>(x[e], base, base * a.c2, a.c2);
+    for (int e = 0; e < n; ++e) l += power(x[e], base, a.c2);
     m = top;
   };
   const uint4 *pieces = reinterpret_cast<const uint4 *>(z + cut.head);
@@ -243,7 +242,7 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_fw
     const float base = top == -__builtin_inff() ? 0.0f : top;
     l *= __builtin_amdgcn_exp2f((m - base) * a.c2);
 #pragma unroll
-    for (int e = 0; e < U * E; ++e) l += power<T>(x[e], base, base * a.c2, a.c2);
+    for (int e = 0; e < U * E; ++e) l += power(x[e], base, a.c2);
     m = top;
   }
   {                                                        // the ends of the row: fewer than E elements each
@@ -286,8 +285,7 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_bw
   if (cut.full > 0) fetch(t - cut.skip);
   te.gather(a, z);
   const bool some = te.sum(a, red);
-  const float base2 = base * a.c2;
-  auto grad = [&](float x) { return some ? f * power<T>(x, base, base2, a.c2) : 0.0f; };
+  auto grad = [&](float x) { return some ? f * power(x, base, a.c2) : 0.0f; };
   for (int i0 = t - cut.skip; i0 < cut.full; i0 += P * U) {
     if (i0 != t - cut.skip) fetch(i0);
 #pragma unroll
@@ -368,13 +366,13 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_fw
     for (int e = 0; e < E; ++e) top = fmaxf(top, y[e]);
   }
   top = row_max<64>(top, nullptr);
-  const float base = top == -__builtin_inff() ? 0.0f : top, base2 = base * a.c2;
-  float l = end ? power<T>(xe, base, base2, a.c2) : 0.0f;
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  float l = end ? power(xe, base, a.c2) : 0.0f;
   for (int i = t; i < cut.full; i += 64) {
     float y[E];
     widen<T>(pieces[i], y);
 #pragma unroll
-    for (int e = 0; e < E; ++e) l += power<T>(y[e], base, base2, a.c2);
+    for (int e = 0; e < E; ++e) l += power(y[e], base, a.c2);
   }
   const float L = row_sum<64>(l, nullptr);
   const bool some = te.sum(a, nullptr);
@@ -404,8 +402,8 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_bw
   row_has_come();
   te.gather(a, x);
   const bool some = te.sum(a, nullptr);
-  const float f = w / L, base2 = base * a.c2;
-  auto grad = [&](float v) { return some ? f * power<T>(v, base, base2, a.c2) : 0.0f; };
+  const float f = w / L;
+  auto grad = [&](float v) { return some ? f * power(v, base, a.c2) : 0.0f; };
   // the gradient takes the logits' place in LDS, its k places are corrected there, and it leaves in whole lines
   uint4 *pieces = reinterpret_cast<uint4 *>(x + cut.head);
   for (int i = t; i < cut.full; i += 64) {

@@ -208,6 +208,51 @@ def test_masked_classes_and_non_finite_values():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('name', TYPES)
+@pytest.mark.parametrize('V', [1000, 5200, 100003])
+@pytest.mark.parametrize('offset', [100.0, 1000.0, -10000.0])
+def test_an_offset_of_the_whole_row_costs_nothing(name, V, offset):
+  """Softmax does not see what all logits of a row have in common: the bounds, which count the row's spread and not its
+  size, hold as they do around zero.  (_make's logits are rounded to the type after the offset is added.)"""
+  import torch
+  z, t, idx, g = _make(41, torch.float32, 9, V, 32)
+  _check((z + offset).to(getattr(torch, name)), t, idx, g, T=0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', TYPES)
+@pytest.mark.parametrize('V', [200, 1000, 6000])
+@pytest.mark.parametrize('offset', [0.0, 300.0, 1000.0, -3000.0])
+def test_loss_of_one_entry_next_to_an_offset(name, V, offset):
+  """One entry: p = 1, loss = T^2 (log L - (z_i - top) / T), so that the row's log L stands alone.  With e = 2^-24 and far the
+  row's spread over T: an exponent's argument (difference, log2(e) / T, product) is off by 3 e far, exp2 by 2 e, a sum of V terms
+  by e (V / 64 + 16); the logarithm, the two divisions and the difference by 4 e (log V + far) + 8 e."""
+  import torch
+  z, t, idx, g = _make(43, torch.float32, 64, V, 1)
+  z, T = (z + offset).to(getattr(torch, name)), 0.5
+  loss, _ = _run(z, t, idx, g, T)
+  want, _, _, _ = _exact(z, t, idx, T, g)
+  x = z.double() / T
+  far = x.amax(1) - x.amin(1)
+  bound = T * T * EPS32 * (3 * far + V / 64 + 18 + 4 * (math.log(V) + far) + 8)
+  off = (loss.double() - want).abs() - bound
+  assert float(off.max()) <= 0, float(off.max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', TYPES)
+@pytest.mark.parametrize('V', [40, 2600, 9000])
+def test_rows_at_the_types_lowest_value(name, V):
+  """Every class of a row masked with the lowest value, or the highest: uniform, as for any other common value."""
+  import torch
+  dtype = getattr(torch, name)
+  z, t, idx, g = _make(42, dtype, 6, V, 4)
+  z[1], z[4] = torch.finfo(dtype).min, torch.finfo(dtype).max
+  for T in (1.0, 0.25):
+    _check(z, t, idx, g, T=T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', TYPES)
 @pytest.mark.parametrize('V', [99, 2500])
 def test_strides_and_alignment(name, V):
   """Rows of a wider buffer, misaligned starts, expanded rows, a transposed view, leading dimensions: the same bits."""
