@@ -689,6 +689,12 @@ variable_list once_differentiable(variable_list grads, const Tensor &a, const Te
   return grads;
 }
 
+// The autograd nodes know no tangents, and a dual tensor need not require a gradient: its primal alone would pass for a constant
+void refuse_tangents(std::initializer_list<const Tensor *> inputs, const char *what) {
+  for (const Tensor *t : inputs)
+    TORCH_CHECK(!t->_fw_grad(0).defined(), what, ": forward-mode differentiation is not supported");
+}
+
 hsgk_attention_args attention_args(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &pad, bool causal,
                                    double scale, const Tensor &out) {
   hsgk_attention_args a{};
@@ -739,6 +745,7 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
     auto sv = ctx->get_saved_variables();
     const Tensor &q = sv[0], &k = sv[1], &v = sv[2], &pad = sv[3], &out = sv[4], &lse = sv[5];
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    refuse_tangents({&grads[0]}, "hsgk::attention");
     const Tensor incoming = grads[0], g = last_contiguous(incoming);
     Tensor dq = at::empty(q.sizes(), q.options()), dk, dv;
     hsgk_attention_args a = attention_args(q, k, v, pad, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), out);
@@ -765,6 +772,7 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
 };
 
 Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, const c10::optional<Tensor> &padding, bool causal, double scale) {
+  refuse_tangents({&q, &k, &v}, "hsgk::attention");
   TORCH_CHECK(q.is_cuda(), "hsgk::attention: tensors must be on a ROCm device (there is no CPU path)");
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
                   q.size(3) == k.size(3) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
@@ -809,6 +817,7 @@ struct TopkDistillFn : public torch::autograd::Function<TopkDistillFn> {
     auto sv = ctx->get_saved_variables();
     const Tensor &z = sv[0], &t = sv[1], &idx = sv[2], &stats = sv[3];
     c10::hip::HIPGuardMasqueradingAsCUDA guard(z.device());
+    refuse_tangents({&grads[0]}, "hsgk::topk_distill");
     const Tensor incoming = grads[0], g = incoming.to(at::kFloat).contiguous();
     Tensor dz = at::empty(z.sizes(), z.options());
     check(hsgk_topk_distill_bwd(z.data_ptr(), type_code(z), z.size(0), z.size(1), z.stride(0), t.data_ptr<float>(),
@@ -820,6 +829,7 @@ struct TopkDistillFn : public torch::autograd::Function<TopkDistillFn> {
 };
 
 Tensor topk_distill(const Tensor &logits, const Tensor &teacher, const Tensor &index, double temperature) {
+  refuse_tangents({&logits, &teacher}, "hsgk::topk_distill");
   TORCH_CHECK(logits.is_cuda(), "hsgk::topk_distill: tensors must be on a ROCm device (there is no CPU path)");
   TORCH_CHECK(logits.dim() == 2 && teacher.dim() == 2 && teacher.sizes() == index.sizes() && teacher.size(0) == logits.size(0) &&
                   (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf) &&

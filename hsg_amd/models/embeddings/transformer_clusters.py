@@ -21,7 +21,7 @@ MAX_HEAD_WIDTH = 128    # include/hsgk.h HSGK_ATTENTION_MAX_WIDTH
 
 
 def attention(query, key, value, key_padding_mask=None, is_causal=False, scale=None):
-  """softmax(scale * query key^T) value per head, differentiable (once) in the three.
+  """softmax(scale * query key^T) value per head, differentiable (once, in reverse mode) in the three.
 
   query [B, L, H, D], key and value [B, S, G, D] with H a multiple of G (query head h uses key head h // (H // G)), all
   float32, bfloat16 or float16 with D <= 128, on one ROCm device; any strides (a last dimension that is not contiguous

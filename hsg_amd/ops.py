@@ -213,6 +213,12 @@ def _once_differentiable(grads, *inputs):
   return tuple(g if g is None else _Once.apply(g, *inputs) for g in grads)
 
 
+def _refuse_tangent(gout):
+  """An incoming gradient with a tangent: its primal alone would pass for a constant (forward refuses by itself: no jvp)."""
+  if torch.autograd.forward_ad.unpack_dual(gout).tangent is not None:
+    raise RuntimeError('attention and topk_distill: forward-mode differentiation is not supported')
+
+
 def _attention_args(q, k, v, padding, causal, scale, out):
   if max(q.shape + k.shape) > 1 << 30:
     raise _lib.HsgkError('attention: a dimension is longer than 2^30')
@@ -257,6 +263,7 @@ class Attention(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, gout):
+    _refuse_tangent(gout)
     q, k, v, padding, out, lse = ctx.saved_tensors
     g = _last_contiguous(gout)
     dev = q.device
@@ -306,6 +313,7 @@ class TopkDistill(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, gloss):
+    _refuse_tangent(gloss)
     z, teacher, index, stats = ctx.saved_tensors
     n, V = z.shape
     g = gloss.to(torch.float32).contiguous()

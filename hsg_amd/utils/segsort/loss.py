@@ -273,7 +273,7 @@ def topk_distillation_loss(logits, teacher_logits, teacher_indices, temperature=
   (an unfilled slot of the retrieval) does not count; a row without any has loss and gradient 0 and still counts as a
   row of the mean.  An index may come more than once.  logits are float32, bfloat16 or float16, rows at any stride; the
   loss is float32 ([...] with reduction 'none', else the 'mean' or 'sum' over the rows), the gradient of `logits`'s type.
-  The teacher receives no gradient: teacher_logits that require one are refused.  Differentiable once."""
+  The teacher receives no gradient: teacher_logits that require one are refused.  Differentiable once, in reverse mode."""
   if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
     raise TypeError('logits must be float32, bfloat16 or float16 (got %s)' % logits.dtype)
   if not teacher_logits.is_floating_point():

@@ -54,6 +54,24 @@ def test_attention_refuses_masks_scales_and_cpu_tensors():
     attention(q, k, v)
 
 
+def test_the_torch_op_refuses_tangents():
+  """(before it looks at the device: no GPU needed)"""
+  import torch
+  import torch.autograd.forward_ad as fwd
+  from hsg_amd import _torch_ops
+  ops = _torch_ops.ops()
+  if ops is None:
+    pytest.skip('the torch binding is not built')
+  with fwd.dual_level():
+    for i in range(3):
+      t = _args()
+      t[i] = fwd.make_dual(t[i], torch.ones_like(t[i]))
+      with torch.no_grad(), pytest.raises(RuntimeError, match='forward-mode'):
+        ops.attention(*t, None, False, 0.5)
+      with pytest.raises(RuntimeError, match='forward-mode'):
+        ops.attention(*t, None, False, 0.5)
+
+
 def test_c_entry_refuses_bad_arguments():
   """The C entry returns -1 with a message before anything is launched."""
   from hsg_amd import _lib
@@ -459,6 +477,42 @@ def test_gradients_cannot_be_differentiated(binding, monkeypatch):
     assert torch.equal(a, b)
     with pytest.raises(RuntimeError, match='differentiable once'):
       torch.autograd.grad(a.sum(), leaves, allow_unused=True, retain_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('binding', ['torch', 'ctypes'])
+def test_tangents_are_refused(binding, monkeypatch):
+  """Forward-mode differentiation raises under both bindings, whether or not the primal requires a gradient; so does a stack that
+  was switched over to the kernels."""
+  import torch
+  import torch.autograd.forward_ad as fwd
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  if binding == 'ctypes':
+    monkeypatch.setenv('HSGK_BINDING', 'ctypes')
+  t, _, _ = _make(5, torch.float32, 2, 9, 11, 2, 2, 16)
+  m = torch.nn.MultiheadAttention(32, 2).cuda()
+  tc.use_attention_kernels(m)
+  x = torch.randn((9, 2, 32), generator=torch.Generator().manual_seed(1)).cuda()
+  for grad in (False, True):
+    for i in range(3):
+      with fwd.dual_level():
+        u = [y.detach().requires_grad_(grad) for y in t]
+        u[i] = fwd.make_dual(u[i], torch.ones_like(u[i]))
+        with pytest.raises(RuntimeError):
+          tc.attention(*u)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+          tc.attention(*u)
+    m.requires_grad_(grad)
+    with fwd.dual_level():
+      y = fwd.make_dual(x, torch.ones_like(x))
+      with pytest.raises(RuntimeError):
+        m(y, y, y)
+  with fwd.dual_level():
+    u = [y.detach().requires_grad_(True) for y in t]
+    out = tc.attention(*u)                                                       # (without a tangent it runs)
+    assert torch.autograd.grad(out, u, torch.ones_like(out), retain_graph=True)[0].shape == t[0].shape
+    with pytest.raises(RuntimeError, match='forward-mode'):                      # a tangent of the incoming gradient
+      torch.autograd.grad(out, u, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
 
 
 @pytest.mark.gpu

@@ -46,6 +46,21 @@ def test_distillation_refuses_cpu_tensors():
   assert '2.00' in repr(TopKDistillationLoss(2.0))
 
 
+def test_the_torch_op_refuses_tangents():
+  """(before it looks at the device: no GPU needed)"""
+  import torch
+  import torch.autograd.forward_ad as fwd
+  from hsg_amd import _torch_ops
+  ops = _torch_ops.ops()
+  if ops is None:
+    pytest.skip('the torch binding is not built')
+  for i in range(2):
+    with fwd.dual_level(), pytest.raises(RuntimeError, match='forward-mode'):
+      t = list(_args().values())
+      t[i] = fwd.make_dual(t[i], torch.ones_like(t[i]))
+      ops.topk_distill(*t, 1.0)
+
+
 def test_c_entry_refuses_bad_arguments():
   from hsg_amd import _lib
   L = _lib.lib()
@@ -330,6 +345,36 @@ def test_gradient_cannot_be_differentiated(binding, monkeypatch):
   assert torch.equal(got, want)
   with pytest.raises(RuntimeError, match='differentiable once'):
     torch.autograd.grad(got.sum(), z)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('binding', ['torch', 'ctypes'])
+def test_tangents_are_refused(binding, monkeypatch):
+  """Forward-mode differentiation raises under both bindings, of the logits and of the teacher."""
+  import torch
+  import torch.autograd.forward_ad as fwd
+  from hsg_amd.utils.segsort.loss import topk_distillation_loss
+  if binding == 'ctypes':
+    monkeypatch.setenv('HSGK_BINDING', 'ctypes')
+  z, t, idx, _ = _make(3, torch.float32, 5, 40, 3)
+  for grad in (False, True):
+    for which in (0, 1):
+      with fwd.dual_level():
+        u = [z.detach().requires_grad_(grad), t.detach()]
+        u[which] = fwd.make_dual(u[which], torch.ones_like(u[which]))
+        for shape in ((5, -1), (1, 5, -1)):
+          v = [x.view(*shape) for x in u] + [idx.view(*shape)]
+          with pytest.raises(RuntimeError):
+            topk_distillation_loss(*v)
+          with torch.no_grad(), pytest.raises(RuntimeError):
+            topk_distillation_loss(*v)
+  with fwd.dual_level():
+    leaf = z.detach().requires_grad_(True)
+    loss = topk_distillation_loss(leaf, t, idx, reduction='none')                # (without a tangent it runs)
+    one = torch.ones_like(loss)
+    assert torch.autograd.grad(loss, leaf, one, retain_graph=True)[0].shape == z.shape
+    with pytest.raises(RuntimeError, match='forward-mode'):                      # a tangent of the incoming gradient
+      torch.autograd.grad(loss, leaf, fwd.make_dual(one, one))
 
 
 @pytest.mark.gpu
