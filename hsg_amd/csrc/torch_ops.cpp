@@ -773,12 +773,13 @@ struct AttentionFn : public torch::autograd::Function<AttentionFn> {
 
 Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v, const c10::optional<Tensor> &padding, bool causal, double scale) {
   refuse_tangents({&q, &k, &v}, "hsgk::attention");
-  TORCH_CHECK(q.is_cuda(), "hsgk::attention: tensors must be on a ROCm device (there is no CPU path)");
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
                   q.size(3) == k.size(3) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
                   (q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) &&
                   k.device() == q.device() && v.device() == q.device(),
               "hsgk::attention: q [B,L,H,D], k and v [B,S,G,D] of one floating type on one device");
+  TORCH_CHECK(k.size(2) >= 1 && q.size(2) % k.size(2) == 0, "hsgk::attention: the query heads are a multiple of the key heads");
+  TORCH_CHECK(q.is_cuda(), "hsgk::attention: tensors must be on a ROCm device (there is no CPU path)");
   Tensor pad = padding.has_value() && padding->defined() ? *padding : Tensor();
   if (pad.defined()) {
     TORCH_CHECK(pad.dim() == 2 && pad.size(0) == k.size(0) && pad.size(1) == k.size(1) && pad.scalar_type() == at::kBool &&

@@ -72,6 +72,21 @@ def test_the_torch_op_refuses_tangents():
         ops.attention(*t, None, False, 0.5)
 
 
+def test_the_torch_op_refuses_heads_that_do_not_divide():
+  """(the op itself, not its Python entry: no key head was a division by zero in the host's code)"""
+  import torch
+  from hsg_amd import _torch_ops
+  ops = _torch_ops.ops()
+  if ops is None:
+    pytest.skip('the torch binding is not built')
+  q, k, v = _args()
+  for query, key, value in ((q, k[:, :, :0], v[:, :, :0]), (q[:, :, :3], k, v)):
+    with pytest.raises(RuntimeError, match='multiple of the key heads'):
+      ops.attention(query.requires_grad_(True), key, value, None, False, 0.5)
+  with pytest.raises(RuntimeError, match='no CPU path'):
+    ops.attention(q, k, v, None, False, 0.5)
+
+
 def test_c_entry_refuses_bad_arguments():
   """The C entry returns -1 with a message before anything is launched."""
   from hsg_amd import _lib
