@@ -831,12 +831,13 @@ struct TopkDistillFn : public torch::autograd::Function<TopkDistillFn> {
 
 Tensor topk_distill(const Tensor &logits, const Tensor &teacher, const Tensor &index, double temperature) {
   refuse_tangents({&logits, &teacher}, "hsgk::topk_distill");
-  TORCH_CHECK(logits.is_cuda(), "hsgk::topk_distill: tensors must be on a ROCm device (there is no CPU path)");
   TORCH_CHECK(logits.dim() == 2 && teacher.dim() == 2 && teacher.sizes() == index.sizes() && teacher.size(0) == logits.size(0) &&
                   (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf) &&
                   teacher.scalar_type() == at::kFloat && index.scalar_type() == at::kLong &&
                   teacher.device() == logits.device() && index.device() == logits.device(),
               "hsgk::topk_distill: logits [n,V], teacher float32 [n,k] and index int64 [n,k] on one device");
+  TORCH_CHECK(teacher.size(1) <= HSGK_DISTILL_MAX_K, "hsgk::topk_distill: at most ", HSGK_DISTILL_MAX_K, " teacher entries a row");
+  TORCH_CHECK(logits.is_cuda(), "hsgk::topk_distill: tensors must be on a ROCm device (there is no CPU path)");
   const Tensor z = last_contiguous(logits), t = teacher.contiguous(), idx = index.contiguous();
   if (at::GradMode::is_enabled() && z.requires_grad()) return TopkDistillFn::apply(z, t, idx, temperature);
   return distill_fwd(z, t, idx, temperature, nullptr);

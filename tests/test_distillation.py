@@ -61,6 +61,21 @@ def test_the_torch_op_refuses_tangents():
       ops.topk_distill(*t, 1.0)
 
 
+def test_the_torch_op_refuses_more_entries_than_32_bits_count():
+  """(the op itself, not its Python entry: 2^32 + 4 entries a row were taken for 4)"""
+  import torch
+  from hsg_amd import _torch_ops
+  ops = _torch_ops.ops()
+  if ops is None:
+    pytest.skip('the torch binding is not built')
+  z, t, idx = _args().values()
+  for k in (257, (1 << 32) + 4):
+    with pytest.raises(RuntimeError, match='at most 256'):
+      ops.topk_distill(z, t[:, :1].expand(3, k), idx[:, :1].expand(3, k), 1.0)
+  with pytest.raises(RuntimeError, match='no CPU path'):
+    ops.topk_distill(z, t, idx, 1.0)
+
+
 def test_c_entry_refuses_bad_arguments():
   from hsg_amd import _lib
   L = _lib.lib()
