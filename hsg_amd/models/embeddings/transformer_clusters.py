@@ -66,7 +66,11 @@ def attention(query, key, value, key_padding_mask=None, is_causal=False, scale=N
 class MultiheadAttention(torch.nn.MultiheadAttention):
   """torch.nn.MultiheadAttention (same parameters, state_dict and call) whose softmax(q k^T) v runs in libhsgk.  Returns
   (output, None): the probabilities are never stored, so there are no weights to return.  A call that needs what the
-  kernels do not offer raises: attn_mask, dropout in training, bias_k / bias_v, add_zero_attn, unbatched inputs."""
+  kernels do not offer raises: attn_mask, dropout in training, bias_k / bias_v, add_zero_attn, unbatched inputs.
+
+  key_padding_mask is bool, or floating point with 0 for a key and -inf for none, which is what torch's own layers make
+  of a bool mask.  Any other value would be added to the scores, which the kernels do not offer; it is not looked for on
+  the host, the outputs of its batch item are NaN."""
 
   def forward(self, query, key, value, key_padding_mask=None, need_weights=False, attn_mask=None,
               average_attn_weights=True, is_causal=False):
@@ -87,6 +91,9 @@ class MultiheadAttention(torch.nn.MultiheadAttention):
     q, k, v = F.linear(query, wq, bq), F.linear(key, wk, bk), F.linear(value, wv, bv)
     if not self.batch_first:                            # [length, batch, channels]: the heads are views, nothing is moved
       q, k, v = q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1)
+    if key_padding_mask is not None and key_padding_mask.is_floating_point():
+      k = k.masked_fill((key_padding_mask != 0)[..., None], math.nan)   # (what a hidden key holds does not matter)
+      key_padding_mask = key_padding_mask == -math.inf
     heads = [t.unflatten(-1, (self.num_heads, self.head_dim)) for t in (q, k, v)]
     out = attention(*heads, key_padding_mask=key_padding_mask, is_causal=is_causal).flatten(2)
     if not self.batch_first:

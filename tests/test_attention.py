@@ -155,6 +155,28 @@ def test_module_refuses_what_the_kernels_do_not_offer():
     drop(x, x, x)
 
 
+@pytest.mark.parametrize('kind', ['encoder', 'decoder'])
+@pytest.mark.parametrize('training', [True, False])
+@pytest.mark.parametrize('batch_first', [True, False])
+def test_torchs_layers_can_be_called_with_padding(kind, training, batch_first):
+  """What use_attention_kernels switches can be called: torch's layers get as far as the device check (they hand a bool mask
+  on as floating point)."""
+  import torch
+  from hsg_amd import _lib
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  x, pad = torch.zeros(2, 6, 32), torch.arange(6)[None] >= torch.tensor([6, 4])[:, None]
+  x = x if batch_first else x.transpose(0, 1)
+  if kind == 'encoder':
+    layer = torch.nn.TransformerEncoderLayer(32, 4, dropout=0.0, batch_first=batch_first).train(training)
+    args, kwargs, n = (x,), {'src_key_padding_mask': pad}, 1
+  else:
+    layer = torch.nn.TransformerDecoderLayer(32, 4, dropout=0.0, batch_first=batch_first).train(training)
+    args, kwargs, n = (x, x), {'tgt_key_padding_mask': pad, 'memory_key_padding_mask': pad}, 2
+  assert tc.use_attention_kernels(layer) == n
+  with pytest.raises(_lib.HsgkError):
+    layer(*args, **kwargs)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the definition in float64 and the bounds
 def _visible(B, L, S, mask, causal, device):
@@ -720,3 +742,64 @@ def test_module_equals_torchs(batch_first):
     assert w is None and a.shape == b.shape
     a, b = a.detach(), b.detach()
     assert float((a.double() - b).norm()) <= 2.0 ** -24 * 400 * float(b.norm())   # three products of 24 .. 48 terms and the rows
+
+
+def _norm_close(got, want, terms):
+  """Norms: 2^-24 * terms of what a chain of float32 products and sums leaves."""
+  a, b = got.detach().double(), want.detach()
+  assert a.shape == b.shape and bool((a - b).isfinite().all())
+  assert float((a - b).norm()) <= 2.0 ** -24 * terms * float(b.norm()), (float((a - b).norm()), float(b.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('training', [True, False])
+@pytest.mark.parametrize('batch_first', [True, False])
+def test_torchs_encoder_layer_with_padding(training, batch_first):
+  """A stock layer that was switched, with a bool mask that torch makes floating point: the rows that count and the gradients
+  of what they add up to equal the unswitched layer's in float64."""
+  import copy
+  import torch
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  torch.manual_seed(3)
+  ours = torch.nn.TransformerEncoderLayer(32, 4, 48, dropout=0.0, batch_first=batch_first).cuda().train(training)
+  plain = copy.deepcopy(ours).double()
+  assert tc.use_attention_kernels(ours) == 1
+  x = torch.randn(3, 20, 32).cuda()
+  pad = (torch.arange(20)[None] >= torch.tensor([20, 13, 1])[:, None]).cuda()
+  w = torch.randn(3, 20, 32).cuda().masked_fill(pad[..., None], 0.0)
+  res = []
+  for net, dtype in ((ours, torch.float32), (plain, torch.float64)):
+    y = x.to(dtype).requires_grad_(True)
+    out = net(y if batch_first else y.transpose(0, 1), src_key_padding_mask=pad)
+    out = out if batch_first else out.transpose(0, 1)
+    g = torch.autograd.grad((out * w.to(dtype)).sum(), [y, net.linear1.weight, net.self_attn.in_proj_weight,
+                                                        net.self_attn.out_proj.weight])
+    res.append([out.masked_fill(pad[..., None], 0.0)] + list(g))
+  # a chain of ten products and norms of at most 60 rows or 48 terms each, whose errors a layer norm may double
+  for a, b in zip(*res):
+    _norm_close(a, b, 2 * 10 * 60)
+
+
+@pytest.mark.gpu
+def test_floating_point_padding_mask():
+  """0 and -inf: the bits of the bool mask, gradients too; any other value: NaN for its batch item and no other."""
+  import torch
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  torch.manual_seed(4)
+  for dtype in (torch.float32, torch.bfloat16):
+    m = torch.nn.MultiheadAttention(32, 4, batch_first=True).cuda().to(dtype)
+    tc.use_attention_kernels(m)
+    x = torch.randn(3, 20, 32).cuda().to(dtype).requires_grad_(True)
+    pad = (torch.arange(20)[None] >= torch.tensor([20, 13, 0])[:, None]).cuda()
+    soft = torch.zeros(pad.shape, device='cuda', dtype=dtype).masked_fill(pad, -math.inf)
+    res = []
+    for mask in (pad, soft):
+      out, _ = m(x, x, x, key_padding_mask=mask)
+      res.append([out] + list(torch.autograd.grad(out.float().square().sum(), [x] + list(m.parameters()))))
+    for a, b in zip(*res):
+      assert torch.equal(a, b)
+    for value in (-1.0, 1.0, torch.finfo(dtype).min, math.inf, math.nan):
+      bad = soft.clone()
+      bad[1, 2] = value
+      out, _ = m(x, x, x, key_padding_mask=bad)
+      assert bool(torch.isnan(out[1]).all()) and torch.equal(out[[0, 2]], res[0][0][[0, 2]])
