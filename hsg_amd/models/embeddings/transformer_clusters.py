@@ -66,7 +66,11 @@ def attention(query, key, value, key_padding_mask=None, is_causal=False, scale=N
 class MultiheadAttention(torch.nn.MultiheadAttention):
   """torch.nn.MultiheadAttention (same parameters, state_dict and call) whose softmax(q k^T) v runs in libhsgk.  Returns
   (output, None): the probabilities are never stored, so there are no weights to return.  A call that needs what the
-  kernels do not offer raises: attn_mask, dropout in training, bias_k / bias_v, add_zero_attn, unbatched inputs.
+  kernels do not offer raises: any other attn_mask than the causal one, dropout in training, bias_k / bias_v,
+  add_zero_attn, unbatched inputs.
+
+  attn_mask [length, length] with is_causal=True, over as many queries as keys, is taken for the causal mask, as is_causal
+  says of it in torch.nn.MultiheadAttention; its values are not read.  is_causal without a mask is `attention`'s.
 
   key_padding_mask is bool, or floating point with 0 for a key and -inf for none, which is what torch's own layers make
   of a bool mask.  Any other value would be added to the scores, which the kernels do not offer; it is not looked for on
@@ -74,14 +78,16 @@ class MultiheadAttention(torch.nn.MultiheadAttention):
 
   def forward(self, query, key, value, key_padding_mask=None, need_weights=False, attn_mask=None,
               average_attn_weights=True, is_causal=False):
-    if attn_mask is not None:
-      raise ValueError('MultiheadAttention: attn_mask is not supported (key_padding_mask and is_causal are)')
     if self.dropout and self.training:
       raise ValueError('MultiheadAttention: dropout of the probabilities is not supported in training')
     if self.bias_k is not None or self.bias_v is not None or self.add_zero_attn:
       raise ValueError('MultiheadAttention: bias_k, bias_v and add_zero_attn are not supported')
     if query.dim() != 3:
       raise ValueError('MultiheadAttention: batched inputs only (got %d dimensions)' % query.dim())
+    if attn_mask is not None:
+      L, S = (t.shape[1 if self.batch_first else 0] for t in (query, key))
+      if not (is_causal and L == S and tuple(attn_mask.shape) == (L, S)):
+        raise ValueError('MultiheadAttention: attn_mask is not supported, but for the [length, length] one with is_causal=True')
     E = self.embed_dim
     if self._qkv_same_embed_dim:
       wq, wk, wv = self.in_proj_weight.split(E)

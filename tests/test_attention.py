@@ -177,6 +177,31 @@ def test_torchs_layers_can_be_called_with_padding(kind, training, batch_first):
     layer(*args, **kwargs)
 
 
+@pytest.mark.parametrize('batch_first', [True, False])
+def test_causal_masks_of_torchs_layers(batch_first):
+  """torch's layers pass a causal mask together with is_causal=True: such a call gets as far as the device check, a mask that
+  is_causal cannot be true of is refused."""
+  import torch
+  from hsg_amd import _lib
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  x, mask = torch.zeros(2, 6, 32), torch.nn.Transformer.generate_square_subsequent_mask(6)
+  y, z = (t if batch_first else t.transpose(0, 1) for t in (x, torch.zeros(2, 8, 32)))
+  enc = torch.nn.TransformerEncoderLayer(32, 4, dropout=0.0, batch_first=batch_first)
+  dec = torch.nn.TransformerDecoderLayer(32, 4, dropout=0.0, batch_first=batch_first)
+  m = torch.nn.MultiheadAttention(32, 4, batch_first=batch_first)
+  assert tc.use_attention_kernels(torch.nn.ModuleList([enc, dec, m])) == 4
+  for call in (lambda: enc(y, src_mask=mask, is_causal=True), lambda: dec(y, y, tgt_mask=mask, tgt_is_causal=True),
+               lambda: m(y, y, y, attn_mask=mask, is_causal=True)):
+    with pytest.raises(_lib.HsgkError):
+      call()
+  for call in (lambda: m(y, y, y, attn_mask=mask), lambda: m(y, z, z, attn_mask=torch.zeros(6, 8), is_causal=True),
+               lambda: m(y, y, y, attn_mask=torch.zeros(8, 8), is_causal=True), lambda: enc(y, src_mask=mask),
+               lambda: m(y, z, z, attn_mask=mask, is_causal=True),
+               lambda: m(y, y, y, attn_mask=torch.zeros(8, 6, 6), is_causal=True)):
+    with pytest.raises(ValueError):
+      call()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the definition in float64 and the bounds
 def _visible(B, L, S, mask, causal, device):
@@ -778,6 +803,29 @@ def test_torchs_encoder_layer_with_padding(training, batch_first):
   # a chain of ten products and norms of at most 60 rows or 48 terms each, whose errors a layer norm may double
   for a, b in zip(*res):
     _norm_close(a, b, 2 * 10 * 60)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('padded', [False, True])
+def test_torchs_decoder_layer_with_causality(padded):
+  """A stock decoder layer: causal self-attention (mask and is_causal), padded keys from elsewhere, against float64."""
+  import copy
+  import torch
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  torch.manual_seed(5)
+  ours = torch.nn.TransformerDecoderLayer(32, 4, 48, dropout=0.0, batch_first=True).cuda()
+  plain = copy.deepcopy(ours).double()
+  assert tc.use_attention_kernels(ours) == 2
+  x, memory, w = torch.randn(3, 20, 32).cuda(), torch.randn(3, 33, 32).cuda(), torch.randn(3, 20, 32).cuda()
+  mask = torch.nn.Transformer.generate_square_subsequent_mask(20).cuda()
+  pad = (torch.arange(33)[None] >= torch.tensor([33, 13, 1])[:, None]).cuda() if padded else None
+  res = []
+  for net, dtype in ((ours, torch.float32), (plain, torch.float64)):
+    y, z = (t.to(dtype).requires_grad_(True) for t in (x, memory))
+    out = net(y, z, tgt_mask=mask.to(dtype), tgt_is_causal=True, memory_key_padding_mask=pad)
+    res.append([out] + list(torch.autograd.grad((out * w.to(dtype)).sum(), [y, z, net.self_attn.in_proj_weight])))
+  for a, b in zip(*res):                                       # fifteen products and norms of at most 60 rows or 48 terms each
+    _norm_close(a, b, 2 * 15 * 60)
 
 
 @pytest.mark.gpu
