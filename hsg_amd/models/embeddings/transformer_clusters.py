@@ -110,11 +110,16 @@ class MultiheadAttention(torch.nn.MultiheadAttention):
 def use_attention_kernels(module):
   """Switches every torch.nn.MultiheadAttention inside `module` (a TransformerClustering, its `_transformer`, a ViT) over
   to MultiheadAttention above, in place and without touching its parameters.  Returns how many were switched; a module
-  that could not be called afterwards (dropout, bias_k, add_zero_attn) raises and nothing is switched."""
+  that could not be called afterwards (dropout in training mode, bias_k / bias_v, add_zero_attn, heads wider than
+  MAX_HEAD_WIDTH) raises and nothing is switched.  One with dropout that is in evaluation mode is switched and raises when
+  it is called in training mode.
+
+  torch.nn.TransformerEncoderLayer in evaluation, with batch_first and without gradients, takes a fused path of torch's own
+  and does not call its attention module; torch.backends.mha.set_fastpath_enabled(False) makes it."""
   found = [m for m in module.modules() if type(m) is torch.nn.MultiheadAttention]
   for m in found:
-    if m.dropout or m.bias_k is not None or m.bias_v is not None or m.add_zero_attn:
-      raise ValueError('use_attention_kernels: an attention module uses dropout, bias_k / bias_v or add_zero_attn')
+    if (m.dropout and m.training) or m.bias_k is not None or m.bias_v is not None or m.add_zero_attn:
+      raise ValueError('use_attention_kernels: an attention module uses dropout in training, bias_k / bias_v or add_zero_attn')
     if m.head_dim > MAX_HEAD_WIDTH:
       raise ValueError('use_attention_kernels: head width %d, at most %d' % (m.head_dim, MAX_HEAD_WIDTH))
   for m in found:

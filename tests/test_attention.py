@@ -202,6 +202,24 @@ def test_causal_masks_of_torchs_layers(batch_first):
       call()
 
 
+def test_dropout_counts_in_training_only():
+  import torch
+  from hsg_amd import _lib
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  x = torch.zeros(6, 2, 32)
+  m = torch.nn.MultiheadAttention(32, 4, dropout=0.1)
+  with pytest.raises(ValueError):
+    tc.use_attention_kernels(m)
+  assert type(m) is torch.nn.MultiheadAttention
+  m.eval()
+  assert tc.use_attention_kernels(m) == 1
+  with pytest.raises(_lib.HsgkError):                        # as far as the device check
+    m(x, x, x)
+  m.train()
+  with pytest.raises(ValueError, match='dropout'):
+    m(x, x, x)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the definition in float64 and the bounds
 def _visible(B, L, S, mask, causal, device):
@@ -826,6 +844,31 @@ def test_torchs_decoder_layer_with_causality(padded):
     res.append([out] + list(torch.autograd.grad((out * w.to(dtype)).sum(), [y, z, net.self_attn.in_proj_weight])))
   for a, b in zip(*res):                                       # fifteen products and norms of at most 60 rows or 48 terms each
     _norm_close(a, b, 2 * 15 * 60)
+
+
+@pytest.mark.gpu
+def test_torchs_encoder_layer_in_evaluation():
+  """With dropout and without gradients, torch's fused path off: the module is called and its rows are torch's."""
+  import copy
+  import torch
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  torch.manual_seed(6)
+  ours = torch.nn.TransformerEncoderLayer(32, 4, 48, dropout=0.1, batch_first=True).cuda().eval()
+  plain = copy.deepcopy(ours).double()
+  assert tc.use_attention_kernels(ours) == 1
+  x = torch.randn(3, 20, 32).cuda()
+  pad = (torch.arange(20)[None] >= torch.tensor([20, 13, 1])[:, None]).cuda()
+  calls = []
+  ours.self_attn.register_forward_hook(lambda *a: calls.append(1))
+  want = plain(x.double().requires_grad_(True), src_key_padding_mask=pad)     # (with gradients: torch's plain path)
+  try:
+    torch.backends.mha.set_fastpath_enabled(False)
+    with torch.no_grad():
+      got = ours(x, src_key_padding_mask=pad)
+  finally:
+    torch.backends.mha.set_fastpath_enabled(True)
+  assert len(calls) == 1
+  _norm_close(got.masked_fill(pad[..., None], 0.0), want.masked_fill(pad[..., None], 0.0), 2 * 6 * 60)
 
 
 @pytest.mark.gpu
