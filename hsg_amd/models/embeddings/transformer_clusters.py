@@ -65,9 +65,9 @@ def attention(query, key, value, key_padding_mask=None, is_causal=False, scale=N
 
 class MultiheadAttention(torch.nn.MultiheadAttention):
   """torch.nn.MultiheadAttention (same parameters, state_dict and call) whose softmax(q k^T) v runs in libhsgk.  Returns
-  (output, None): the probabilities are never stored, so there are no weights to return.  A call that needs what the
-  kernels do not offer raises: any other attn_mask than the causal one, dropout in training, bias_k / bias_v,
-  add_zero_attn, unbatched inputs.
+  (output, None): the probabilities are never stored, so there are no weights to return (and need_weights is False unless
+  it is asked for).  A call that needs what the kernels do not offer raises: need_weights=True, any other attn_mask than
+  the causal one, dropout in training, bias_k / bias_v, add_zero_attn, unbatched inputs.
 
   attn_mask [length, length] with is_causal=True, over as many queries as keys, is taken for the causal mask, as is_causal
   says of it in torch.nn.MultiheadAttention; its values are not read.  is_causal without a mask is `attention`'s.
@@ -78,6 +78,8 @@ class MultiheadAttention(torch.nn.MultiheadAttention):
 
   def forward(self, query, key, value, key_padding_mask=None, need_weights=False, attn_mask=None,
               average_attn_weights=True, is_causal=False):
+    if need_weights:
+      raise ValueError('MultiheadAttention: need_weights=True is not supported, the probabilities are never stored')
     if self.dropout and self.training:
       raise ValueError('MultiheadAttention: dropout of the probabilities is not supported in training')
     if self.bias_k is not None or self.bias_v is not None or self.add_zero_attn:

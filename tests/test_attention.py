@@ -220,6 +220,21 @@ def test_dropout_counts_in_training_only():
     m(x, x, x)
 
 
+def test_weights_that_are_asked_for_are_refused():
+  """(they were None without a word)"""
+  import torch
+  from hsg_amd import _lib
+  from hsg_amd.models.embeddings import transformer_clusters as tc
+  x = torch.zeros(6, 2, 32)
+  m = torch.nn.MultiheadAttention(32, 4)
+  tc.use_attention_kernels(m)
+  with pytest.raises(ValueError, match='need_weights'):
+    m(x, x, x, need_weights=True)
+  for kwargs in ({}, {'need_weights': False}):
+    with pytest.raises(_lib.HsgkError):                      # as far as the device check
+      m(x, x, x, **kwargs)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the definition in float64 and the bounds
 def _visible(B, L, S, mask, causal, device):
