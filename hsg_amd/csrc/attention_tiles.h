@@ -178,9 +178,12 @@ __device__ __forceinline__ void rare() { asm volatile("; rare"); }
 
 // Streamed rows go from memory straight into LDS, 16 bytes a lane (a wave fills 1 KB in lane order, so a lane fetches the
 // piece that belongs into its place); no register holds them on the way.  Written as an instruction because the compiler
-// would wait for it at the next LDS read, whichever buffer that reads; the loop waits itself (stream()).
+// would wait for it at the next LDS read, whichever buffer that reads; the loop waits itself (stream()).  m0, which holds the
+// place, is the compiler's and is put back (it cannot be named as clobbered).
 __device__ __forceinline__ void load_to_lds(const void *from, uint32_t lds_byte) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_byte), "v"(from) : "memory");
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "s"(lds_byte), "v"(from) : "memory");
 }
 // (the builtin, not an instruction of ours: the compiler then knows that its own loads from before the loop have arrived and
 //  does not wait for them -- and so for the tile under way -- at their first use inside it)

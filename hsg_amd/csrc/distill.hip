@@ -312,8 +312,13 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void distill_bw
 // length and not U bounds what is under way, and the teacher's k places are read there: in memory those reads touched
 // nearly half of a row's lines a second time.
 template <bool NT> __device__ __forceinline__ void row_to_lds(const void *from, uint32_t lds_byte) {
-  if (NT) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_byte), "v"(from) : "memory");
-  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_byte), "v"(from) : "memory");
+  uint32_t m0;                                             // (the compiler's: put back)
+  if (NT)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(lds_byte), "v"(from) : "memory");
+  else
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(lds_byte), "v"(from) : "memory");
 }
 
 // bytes of LDS of a row: 128 in front (the head and the line's start), whole pieces, the rest

@@ -214,3 +214,22 @@ def test_bench_roofline_byte_sources_come_from_the_newest_counter_pass():
     e_bytes = bench.pmc_traffic('assign', wl)[0] / n
     assert e_bytes < 4 * d + 8, 'the filtered E-step moves less than one fp32 read of every row'
   assert bench.pmc_traffic('assign', 'cfg1') == (None, None, None, None)
+
+
+def test_inline_assembly_puts_m0_back():
+  """An asm statement that writes m0 saves it first and ends by restoring it: the compiler keeps values of its own there
+  (indexed register moves, its own loads into LDS), and as a reserved register m0 cannot be listed as clobbered."""
+  csrc = os.path.join(ROOT, 'hsg_amd', 'csrc')
+  seen = 0
+  for name in sorted(os.listdir(csrc)):
+    if not name.endswith(('.hip', '.h', '.cpp')):
+      continue
+    text = open(os.path.join(csrc, name)).read()
+    for stmt in re.findall(r'\basm\s+volatile\s*\(.*?\);', text, re.S):
+      code = ''.join(re.findall(r'"((?:[^"\\]|\\.)*)"', stmt.split(':')[0])).split('\\n\\t')
+      writes = [i for i, line in enumerate(code) if re.match(r's_\w+ m0\b', line)]
+      if writes:
+        seen += 1
+        keep = re.match(r's_mov_b32 (%\d), m0$', code[0])
+        assert keep and code[-1] == 's_mov_b32 m0, %s' % keep.group(1) and writes[0] > 0, (name, code)
+  assert seen
