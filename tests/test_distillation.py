@@ -250,6 +250,24 @@ def test_an_offset_of_the_whole_row_costs_nothing(name, V, offset):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('name', TYPES)
+@pytest.mark.parametrize('more', [-1, 0, 1])
+@pytest.mark.parametrize('lead', [0, 1, 3])
+def test_longest_rows_that_go_through_lds(name, more, lead):
+  """One class either side of 10 KB, where a workgroup takes over from a wave, with the most entries, row starts that are
+  aligned or not, and a last workgroup that is not full."""
+  import torch
+  dtype = getattr(torch, name)
+  V = 10240 // torch.empty((), dtype=dtype).element_size() + more
+  z, t, idx, g = _make(44, dtype, 7, V, 256)
+  idx[:, :4] = torch.tensor([0, V - 1, 0, V - 1])                    # both ends of the row, twice
+  wide = torch.full((7, V + 5), math.nan, dtype=dtype, device='cuda')
+  view = wide[:, lead:lead + V]
+  view.copy_(z)
+  _check(view, t, idx, g, T=2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', TYPES)
 @pytest.mark.parametrize('V', [200, 1000, 6000])
 @pytest.mark.parametrize('offset', [0.0, 300.0, 1000.0, -3000.0])
 def test_loss_of_one_entry_next_to_an_offset(name, V, offset):
