@@ -609,7 +609,9 @@ void attn_fwd_kernel(const AttnArgs a) {
     top = both_max(top);
     const float mn = fmaxf(m, top);
     if (__any((mn - m) * a.c2 > kAttnLazy)) {                         // (a column whose maximum stays: factor 1)
-      const float f = mn > m ? exp2f((m - mn) * a.c2) : 1.0f;
+      // (the difference of the two references as they are rounded below: of scores around 3000 whose parts are joined here,
+      //  exp2((m - mn) c2) would weigh one against the other by 1.5e-4 too much or too little)
+      const float f = !(mn > m) ? 1.0f : m == -__builtin_inff() ? 0.0f : exp2f((fwd_shift<T>() - mn * a.c2) - (fwd_shift<T>() - m * a.c2));
       l *= f;
 #pragma unroll
       for (int db = 0; db < Ti::DB; ++db)

@@ -419,6 +419,32 @@ def test_attention_scales_and_large_scores(name):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('offset', [0.0, 300.0, 3000.0, -30000.0])
+@pytest.mark.parametrize('B, L, H', [(1, 1, 1), (1, 200, 2), (16, 130, 16), (1, 40, 1)])
+def test_an_offset_of_all_scores_costs_nothing(B, L, H, offset):
+  """Width 1 and queries of 1, so that the scores are the keys, without rounding.  What they have in common leaves the softmax,
+  and the parts of a row that is summed in steps weigh alike: keys that grow by 10 once a tile with values that shrink as much.
+
+  With e = 2^-24 and far the spread of the scores: an argument (s log2(e) fused with a reference, log2(e) rounded, the same
+  reference throughout) is off by 4 e far, exp2 by 2 e here and 2 e for each of up to eight rescalings and joins, a sum of S terms
+  by e S, twice (numerator and denominator), the value's product and the division by 4 e."""
+  import torch
+  from hsg_amd.models.embeddings.transformer_clusters import attention
+  S = 700
+  gen = torch.Generator().manual_seed(51)
+  step = torch.arange(S) // 130
+  k = (offset + 10.0 * step + torch.rand((B, S), generator=gen))
+  v = (1.0 + torch.rand((B, S), generator=gen)) * torch.exp(-10.0 * step.double()).float()
+  k, v = k[:, :, None, None].cuda(), v[:, :, None, None].cuda()
+  out = attention(torch.ones((B, L, H, 1), device='cuda'), k.expand(B, S, H, 1), v.expand(B, S, H, 1), scale=1.0)
+  s = k[:, :, 0, 0].double()
+  want = (torch.softmax(s, 1) * v[:, :, 0, 0].double()).sum(1)
+  far = float((s.amax(1) - s.amin(1)).max())
+  off = (out.double() - want[:, None, None, None]).abs() / want[:, None, None, None]
+  assert float(off.max()) <= EPS32 * 2 * (4 * far + 2 + 16 + S + 4), float(off.max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('name', TYPES)
 @pytest.mark.parametrize('shape', [
     (2, 9, 1, 2, 1, 24, None, False),
