@@ -29,8 +29,12 @@ def attention(query, key, value, key_padding_mask=None, is_causal=False, scale=N
   may hold anything, NaN included.  is_causal: query i sees the keys j <= i + S - L (the last query sees every key).
   scale: positive, 1 / sqrt(D) when None.  Returns [B, L, H, D], contiguous, of the inputs' type.
 
-  A query that sees no key has output 0 and passes no gradient (torch's softmax gives NaN there).  Sums, statistics and
-  probabilities are float32; the backward pass recomputes the probabilities, uses no atomics and repeats bit for bit.
+  A query that sees no key has output 0 and passes no gradient (torch's softmax gives NaN there).  Sums and statistics are
+  float32; between 16-bit inputs a probability, and its gradient, is rounded to their type where it enters the second
+  product, so that an output is off by about 1.4 roundings and not one.  A score is float32 too: a probability's relative
+  error is 2^-23 of the row's largest score or so, and scores past 2^22 leave float16's range.  Causality hides what is
+  finite: a NaN or an infinity in a row that some query of the batch item sees may reach queries next to it that do not.
+  The backward pass recomputes the probabilities, uses no atomics and repeats bit for bit.
   Under graph capture take gradients with torch.autograd.grad, which adds nothing to leaves that another graph holds.
   """
   for name, t in (('query', query), ('key', key), ('value', value)):

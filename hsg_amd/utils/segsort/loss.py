@@ -264,7 +264,7 @@ MAX_TEACHER_ENTRIES = 256      # include/hsgk.h HSGK_DISTILL_MAX_K
 def topk_distillation_loss(logits, teacher_logits, teacher_indices, temperature=1.0, reduction='mean'):
   """Distillation of a softmax over the last dimension of `logits` [..., V] (a pixel's similarities to V prototypes) from
   a teacher of whom only the k best are known: `teacher_logits` and `teacher_indices` [..., k], as
-  `utils.segsort.eval.top_k_indices` returns them (values and indices).
+  `utils.segsort.eval.top_k_indices` returns them (the other way round: indices, then values).
 
     p = softmax(teacher_logits / T) over the k entries,  q = softmax(logits / T) over all V
     loss = T^2 sum_j p_j (log p_j - log q_index_j)

@@ -501,11 +501,14 @@ HSGK_API int hsgk_synth_mixture(uint64_t noise_key, uint64_t seed, const float *
  *   out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys that query i sees
  * A key with padding[b][j] != 0 (padding uint8 [B,S], batch stride padding_stride, nullable) is seen by no query and its
  * k and v rows may hold anything; with `causal` query i sees the keys j <= i + S - L (the last query sees all).  A query
- * that sees no key, or only scores of -inf, has output 0 and passes no gradient.
+ * that sees no key, or only scores of -inf (products past float32's range; an infinite element makes gradients NaN), has
+ * output 0 and passes no gradient.  Causality hides what is finite: a NaN or an infinity in a row that some query sees may
+ * reach queries next to it that do not see it.
  * dtype 0 float32, 1 bfloat16, 2 float16; sums, statistics and probabilities are float32, a probability (and its gradient)
  * is rounded to the 16-bit type where it enters a product of that type.  Strides are in elements: {batch, row, head};
  * the last dimension is contiguous; out, dq, dk and dv are contiguous and 16-byte aligned.  1 <= D <= 128, scale > 0.
- * lse float32 [B,G,L,H/G] (forward: nullable; backward: what the forward wrote): log2 of the sum of 2^(score log2 e).
+ * lse float32 [B,G,L,H/G] (forward: nullable; backward: what the forward wrote): log2 of the sum of 2^(score log2 e), whose
+ * rounding (2^-24 of its size) the recomputed probabilities carry.  In float16 |score| has to stay below 2^22.
  * backward: reads out and lse of the forward, recomputes the probabilities, writes dq and (both or neither) dk, dv; no
  * atomics, the order of every sum is fixed.  The backward sums delta = sum_j p_j (dout_i . v_j) in float32 where a query
  * sees few keys, and takes dout_i . out_i elsewhere.
