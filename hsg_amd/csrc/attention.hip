@@ -8,7 +8,7 @@ namespace hsgk {
 
 static int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 // (float32, whose products cost seven times as much, also to 96: 30 heads x 930 x 930, width 72, forward, dq, dk and dv 123 + 169 +
-// 222 us, 150 + 210 + 275 with 128)
+// 222 us, 150 + 210 + 275 with 128; the 16-bit types have no such form, nor one of 48: not measured)
 static int padded_width(const hsgk_attention_args &a) {
   return a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.dtype == 0 && a.D <= 96 ? 96 : 128;
 }
@@ -26,7 +26,8 @@ struct AttnPlan {
 // 117).
 // Split rows where there are fewer workgroups than `room`, what the CUs hold at a time: more only add partial results (one token of
 // 16 heads over 2 x 32768 keys, width 128: 256 workgroups 25 + 4 us, 512 30 + 4; 30 heads x 930 x 930, width 72, float32, 240
-// workgroups 143 us, 480 153 + 9).  Causal blocks differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys:
+// workgroups 143 us, 480 153 + 9; narrower 16-bit heads, whose workgroups fit three times on a CU, have the same room without
+// a measurement of their own).  Causal blocks differ in length: two for each CU there (dk and dv of 4 key heads, 8192 keys:
 // 1105 us in one part, 760 + 16 in two).
 static AttnPlan attn_plan(const hsgk_attention_args &a, AttnPass pass) {
   const bool dkv = pass == kAttnDkv;

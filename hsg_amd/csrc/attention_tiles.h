@@ -529,11 +529,11 @@ template <typename T, int DP, int TR> struct KeyRows {
   __device__ __forceinline__ uint32_t bits_of(int r0, int h) const { return (uint32_t)(word(r0 >> 6) >> ((r0 & 63) + 4 * h)); }
 };
 // ---------------------------------------------------------------------------------------------------------------------
-// forward: columns = queries, keys and values stream.  Long sequences are bound by the matrix and the vector unit in turn (of
-// the two waves of a SIMD one rarely multiplies while the other takes its exponentials): 24 heads x 2305 x 2305, width 64,
-// bfloat16, 57 us, 570 TFLOP/s; 16 heads x 8192 x 8192 causal, width 128, 295 us, 930 TFLOP/s (a large matrix product 1130);
-// float32 is bound by its matrix instructions.  Few queries are bound by the keys and values: one token of 16 heads on 4, 2 x
-// 32768 keys, width 128, 26 + 4 us, 5.1 TB/s (a large copy 5.2).
+// forward: columns = queries, keys and values stream.  Long sequences are bound by the matrix and the vector unit in turn (a
+// wave multiplies or takes exponentials, and few waves share a SIMD: 1.3 and 1.6 on average in the next two), medians of ten: 24
+// heads x 2305 x 2305, width 64, bfloat16, 57 us, 570 TFLOP/s; 16 heads x 8192 x 8192 causal, width 128, 295 us, 930 TFLOP/s (a
+// large matrix product 1130).  float32 adds matrix instructions of an eighth of the rate.  Few queries are bound by the keys and
+// values: one token of 16 heads on 4, 2 x 32768 keys, width 128, 25 + 5 us, 5.2 TB/s (a large copy 5.2).
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))
 void attn_fwd_kernel(const AttnArgs a) {
@@ -761,7 +761,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_fwd_jo
 
 // ---------------------------------------------------------------------------------------------------------------------
 // dq, or with SUM delta alone: columns = queries, keys and values stream; three products, bound like the forward pass (the
-// two shapes there: 70 us, 700 TFLOP/s, and 405 us, 1020 TFLOP/s)
+// two shapes there: 75 us, 650 TFLOP/s, and 413 us, 1000 TFLOP/s)
 //
 // delta = do . o carries the rounding of a 16-bit o: as much as one of do . v, while what is left of dp - delta over few
 // keys is no more (relative error of dq against 64 bits, where rounding the exact dq gives 1: 2.3 for 2 keys, 1.55 for 16,
@@ -922,8 +922,9 @@ void attn_dq_kernel(const AttnArgs a) {
 // ---------------------------------------------------------------------------------------------------------------------
 // dk and dv: columns = keys, the queries that use this key head and their output gradients stream; the heads of a group are
 // rows of the same stream, so shared heads are summed here, in a fixed order and without atomics.  Four products; the two
-// shapes above: 85 us, 770 TFLOP/s, and 750 us, 730 TFLOP/s (at width 128 the sums of dk and dv leave registers for one wave
-// a SIMD, which waits for its own exponentials).
+// shapes above: 89 us, 730 TFLOP/s, and 784 us, 700 TFLOP/s (at width 128 the sums of dk and dv leave registers for one wave
+// a SIMD, which waits for its own exponentials).  Shared columns at width 128 do not fit the registers: float32 spills 173 of
+// 512 (16 heads x 256 x 256: 40 us beside 22 for forward and 27 for dq), the 16-bit types 17 and 20 (16 us beside 14 and 11).
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WB)))
 void attn_dkv_kernel(const AttnArgs a) {
