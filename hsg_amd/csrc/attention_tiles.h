@@ -532,7 +532,7 @@ template <typename T, int DP, int TR> struct KeyRows {
 // forward: columns = queries, keys and values stream.  Long sequences are bound by the matrix and the vector unit in turn (a
 // wave multiplies or takes exponentials, and few waves share a SIMD: 1.3 and 1.6 on average in the next two), medians of ten: 24
 // heads x 2305 x 2305, width 64, bfloat16, 57 us, 570 TFLOP/s; 16 heads x 8192 x 8192 causal, width 128, 295 us, 930 TFLOP/s (a
-// large matrix product 1130).  float32 adds matrix instructions of an eighth of the rate.  Few queries are bound by the keys and
+// large matrix product 1130).  float32 adds matrix instructions of a seventh of the rate.  Few queries are bound by the keys and
 // values: one token of 16 heads on 4, 2 x 32768 keys, width 128, 25 + 5 us, 5.2 TB/s (a large copy 5.2).
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Shape<T, DP, KW>::WF)))

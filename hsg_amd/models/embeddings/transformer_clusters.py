@@ -78,7 +78,7 @@ class MultiheadAttention(torch.nn.MultiheadAttention):
 
   key_padding_mask is bool, or floating point with 0 for a key and -inf for none, which is what torch's own layers make
   of a bool mask.  Any other value would be added to the scores, which the kernels do not offer; it is not looked for on
-  the host, the outputs of its batch item are NaN."""
+  the host: a query that sees such a key gets NaN."""
 
   def forward(self, query, key, value, key_padding_mask=None, need_weights=False, attn_mask=None,
               average_attn_weights=True, is_causal=False):
